@@ -35,6 +35,11 @@ extern "C" {
 #define CBMOE_DEVERR_INDEX 2       /* an expert id >= E was routed (the slot is skipped); ids < 0 are empty slots */
 #define CBMOE_DEVERR_CAPACITY 4    /* expert parallel: more slots for one peer than the capacity (extra dropped) */
 
+#define CBMOE_BF16 0               /* element types of the entry points that take one */
+#define CBMOE_F16 1
+#define CBMOE_F32 2
+#define CBMOE_E4M3 3               /* 8-bit floating point, with scales (cbmoe_fp8_linear's x) */
+
 #define CBMOE_PATH_AUTO 0          /* decode kernel for small batches, grouped tensor-core GEMM otherwise */
 #define CBMOE_PATH_DECODE 1        /* fused dequant matvec (resident.py:110-120 `_apply_kernel`) */
 #define CBMOE_PATH_GROUPED 2       /* grouped dequant GEMM (resident.py:144-165 `_apply_ragged_kernel`) */
@@ -224,6 +229,63 @@ int cbmoe_ep_peer_destroy(void* peer);
  * normalized to sum 1 when norm_topk (w / (sum + 1e-20)), times scaling. E <= 256, k <= 32, k <= E. */
 int cbmoe_route(const uint16_t* x, int N, int D, const uint16_t* router_w, const float* bias, int E, int k,
                 int norm_topk, float scaling, int32_t* idx, float* w, cudaStream_t stream);
+
+/* ------------------------------------------------------------------------- 8-bit floating point (e4m3)
+ * Weights as block-scaled checkpoints hold them (the reference's loader reads such safetensors, checkpoint.py): e4m3
+ * codes [rows][K] and one fp32 scale per 128 x 128 block, [ceil(rows/128)][ceil(K/128)]; the row stride (bytes, a
+ * multiple of 16, >= K) is an argument, the first row 16-byte aligned, the scales dense. Activations are quantised per
+ * row in groups of 128 columns: scale = the least power of two s >= 2^-100 with max|x| <= 448 s, codes = e4m3(x / s)
+ * (an exact division; round to nearest even); a group that holds an infinity or a NaN has the scale NaN and stands for
+ * NaN, so the row's products are NaN. Any rows >= 1 and K >= 1: sizes need not be multiples of anything.
+ * No counterpart in the reference, which converts such weights to other formats at load time. */
+/* x [N][K] of `type` (CBMOE_BF16 / F16 / F32; row stride ldx elements) -> q [N][K] e4m3 (row stride ldq bytes; bytes
+ * between K and ldq may be written with zeros) and s fp32 [N][ceil(K/128)]. */
+int cbmoe_fp8_quantize(const void* x, int type, int N, int K, long long ldx, uint8_t* q, long long ldq, float* s,
+                       cudaStream_t stream);
+/* y [N][rows] (y_type) = x W^T, W = e4m3 codes q with scales s. x: bf16, fp16 or fp32 (quantised here, xs NULL), or
+ * CBMOE_E4M3 codes with their scales xs [N][ceil(K/128)] as cbmoe_fp8_quantize makes them (any fp32 scales; ldx a
+ * multiple of 16, x 16-byte aligned). fp32 sums. Workspace: the query (256-byte aligned; zero bytes for
+ * CBMOE_E4M3 input below a size that needs partial sums). */
+size_t cbmoe_fp8_linear_workspace_bytes(int N, int K, int rows, int x_type);
+int cbmoe_fp8_linear(const void* q, long long ldq, const float* s, int rows, int K, const void* x, int x_type,
+                     long long ldx, const float* xs, int N, void* y, int y_type, void* workspace,
+                     size_t workspace_bytes, cudaStream_t stream);
+/* Routed experts on such tables, behind the same boundary as cbmoe_experts_apply (resident.py:100-120): gate, up
+ * [E][I][ld_in], down [E][H][ld_down] with scales [E][ceil(I/128)][ceil(H/128)] and [E][ceil(H/128)][ceil(I/128)].
+ * x bf16 [N][H], idx int32 [N][k] (negative: empty slot), w fp32 [N][k] -> y [N][H] of y_type =
+ * sum_j w[n, j] down_e(swiglu_clamped(gate_e x_n, up_e x_n, limit)); x and the SwiGLU output are quantised as above.
+ * Each slot's output is rounded to y_type before the weighted fp32 sum. E <= 1024, k <= 64. */
+typedef struct {
+  int E, H, I;
+  const void* gate;
+  const void* up;
+  const void* down;
+  const float* gate_s;
+  const float* up_s;
+  const float* down_s;
+  long long ld_in;             /* row stride of gate and up, bytes */
+  long long ld_down;
+} cbmoe_fp8_experts;
+size_t cbmoe_fp8_experts_workspace_bytes(const cbmoe_fp8_experts* ex, int N, int k, int y_type);
+int cbmoe_fp8_experts_apply(const cbmoe_fp8_experts* ex, const uint16_t* x, int N, const int32_t* idx, const float* w,
+                            int k, float limit, void* y, int y_type, void* workspace, size_t workspace_bytes,
+                            cudaStream_t stream);
+
+/* ------------------------------------------------------------------- tokens into expert order and back
+ * Over a routing plan's row_slot [T][k] (a slot's sorted row; outside [0, R): empty) and tok_row [R] (a sorted row's
+ * token; < 0: padding). Element type CBMOE_BF16 / F16 / F32, rows dense [.][H], any H; sums in fp32 over j in order,
+ * rounded once, no atomics. The row gather and the combine of resident.py:144-165 as operators, with gradients. */
+/* xs[row_slot[t][j]] = x[t]; rows with tok_row < 0 are zero. Its gradient is cbmoe_unpermute with w NULL. */
+int cbmoe_permute(const void* x, int type, int T, int H, const int32_t* row_slot, int k, const int32_t* tok_row, int R,
+                  void* xs, cudaStream_t stream);
+/* y[t] = sum_j w[t][j] * ys[row_slot[t][j]] (w fp32, NULL: ones). */
+int cbmoe_unpermute(const void* ys, int type, int R, int H, const int32_t* row_slot, const float* w, int T, int k,
+                    void* y, cudaStream_t stream);
+/* Gradients of cbmoe_unpermute: dys[row_slot[t][j]] = w[t][j] * dy[t] (zero where tok_row < 0), dw[t][j] =
+ * <dy[t], ys[row_slot[t][j]]> (0 for an empty slot). dys or dw may be NULL; ys is read for dw only. */
+int cbmoe_unpermute_backward(const void* dy, const void* ys, int type, int R, int H, const int32_t* row_slot,
+                             const int32_t* tok_row, const float* w, int T, int k, void* dys, float* dw,
+                             cudaStream_t stream);
 
 /* ---- llama.cpp IQ expert formats (the reference's real GLM-5.3-Flash tables) ----------------------------------
  * Raw GGUF blocks of 256 weights, identified by their ggml_type numbers. Replaces iqquant.dequant_rows

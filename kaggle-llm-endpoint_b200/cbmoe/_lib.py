@@ -9,6 +9,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libcbmoe.so")
 
 c_int, c_float, c_size_t, c_void_p, c_int64 = ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_int64
+c_longlong = ctypes.c_longlong
 
 PATHS = {"auto": 0, "decode": 1, "grouped": 2}
 
@@ -33,6 +34,16 @@ class IqExperts(ctypes.Structure):
                 ("gate_table", c_void_p), ("up_table", c_void_p), ("down_table", c_void_p),
                 ("gate8", c_void_p), ("up8", c_void_p), ("down8", c_void_p)]
 
+
+class Fp8Experts(ctypes.Structure):
+    _fields_ = [("E", c_int), ("H", c_int), ("I", c_int), ("gate", c_void_p), ("up", c_void_p), ("down", c_void_p),
+                ("gate_s", c_void_p), ("up_s", c_void_p), ("down_s", c_void_p), ("ld_in", ctypes.c_longlong),
+                ("ld_down", ctypes.c_longlong)]
+
+
+# element types (CBMOE_BF16, ...) of the entry points that take one
+TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+E4M3 = 3
 
 # name: (restype, argtypes)
 SIGNATURES = {
@@ -94,6 +105,17 @@ SIGNATURES = {
     "cbmoe_iq_workspace_bytes": (c_size_t, [ctypes.POINTER(IqExperts), c_int, c_int]),
     "cbmoe_iq_experts_apply": (c_int, [ctypes.POINTER(IqExperts), c_void_p, c_int, c_void_p, c_void_p, c_int, c_float,
                                        c_void_p, c_void_p, c_size_t, c_void_p]),
+    "cbmoe_fp8_quantize": (c_int, [c_void_p, c_int, c_int, c_int, c_longlong, c_void_p, c_longlong, c_void_p, c_void_p]),
+    "cbmoe_fp8_linear_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "cbmoe_fp8_linear": (c_int, [c_void_p, c_longlong, c_void_p, c_int, c_int, c_void_p, c_int, c_longlong, c_void_p,
+                                 c_int, c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
+    "cbmoe_fp8_experts_workspace_bytes": (c_size_t, [ctypes.POINTER(Fp8Experts), c_int, c_int, c_int]),
+    "cbmoe_fp8_experts_apply": (c_int, [ctypes.POINTER(Fp8Experts), c_void_p, c_int, c_void_p, c_void_p, c_int, c_float,
+                                        c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
+    "cbmoe_permute": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p]),
+    "cbmoe_unpermute": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p]),
+    "cbmoe_unpermute_backward": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int,
+                                         c_int, c_void_p, c_void_p, c_void_p]),
 }
 
 _lib = None

@@ -7,7 +7,7 @@ import ctypes
 
 import torch
 
-from ._lib import check, lib, ptr, require_cuda, stream_handle
+from ._lib import E4M3, TYPES, check, lib, ptr, require_cuda, stream_handle
 
 PLAN_FIELDS = ("counts", "row_start", "act", "n_act", "n_blocks", "n_pass", "blk_expert", "tok_row", "w_row",
                "row_slot", "pass_expert", "pass_row0", "pass_cnt")
@@ -157,3 +157,106 @@ def w8_logits(qk, s, rows, K, x, ws=None):
                                 ws.numel(), stream_handle()), "cbmoe_w8_logits")
     return out
 
+
+def _fp8_x(x):
+    """(x 2-D with unit inner stride, its row stride in elements)."""
+    if x.dim() != 2:
+        raise ValueError(f"x is [N, K], got {tuple(x.shape)}")
+    if x.stride(1) != 1 or x.stride(0) < x.shape[1]:
+        x = x.contiguous()
+    return x, max(x.stride(0), x.shape[1])
+
+
+def fp8_quantize(x):
+    """x [N, K] (bf16, fp16 or fp32) -> (q float8_e4m3fn [N, K], s fp32 [N, ceil(K / 128)]): per row and group of 128
+    columns the scale is the least power of two s >= 2^-100 with max|x| <= 448 s, the codes e4m3(x / s). A group with
+    an infinity or a NaN has the scale NaN. q is a view of rows padded to 16 bytes, as fp8_linear takes it."""
+    require_cuda(x)
+    if x.dtype not in TYPES:
+        raise ValueError(f"x is bf16, fp16 or fp32, got {x.dtype}")
+    x, ldx = _fp8_x(x)
+    N, K = x.shape
+    if K == 0:
+        raise ValueError("x has no columns")
+    ld = -(-K // 16) * 16
+    with torch.cuda.device(x.device):
+        q = torch.empty((N, ld), dtype=torch.float8_e4m3fn, device=x.device)
+        s = torch.empty((N, -(-K // 128)), dtype=torch.float32, device=x.device)
+        check(lib().cbmoe_fp8_quantize(ptr(x), TYPES[x.dtype], N, K, ldx, ptr(q), ld, ptr(s), stream_handle()),
+              "cbmoe_fp8_quantize")
+    return q[:, :K], s
+
+
+def fp8_pad_rows(q):
+    """e4m3 codes [.., rows, K] in the layout the kernels read: unit inner stride, rows dense at a stride of a multiple
+    of 16 bytes, first row 16-byte aligned. Returned as they are when they already are so; else a padded copy (load time)."""
+    if q.dtype != torch.float8_e4m3fn or q.dim() < 2:
+        raise ValueError(f"codes are float8_e4m3fn [.., rows, K], got {q.dtype} {tuple(q.shape)}")
+    K = q.shape[-1]
+    if fp8_row_stride(q) is not None:
+        return q
+    out = torch.zeros(q.shape[:-1] + (-(-K // 16) * 16,), dtype=torch.uint8, device=q.device)
+    out[..., :K] = q.view(torch.uint8) if q.stride(-1) == 1 else q.contiguous().view(torch.uint8)
+    return out.view(torch.float8_e4m3fn)[..., :K]
+
+
+def fp8_row_stride(q):
+    """Row stride (bytes) of codes laid out as the kernels read them (fp8_pad_rows), or None."""
+    ld = q.stride(-2) if q.shape[-2] > 1 else -(-q.shape[-1] // 16) * 16
+    if q.shape[-2] == 1 and q.dim() == 3 and q.shape[0] > 1:
+        ld = q.stride(0)
+    ok = (q.stride(-1) == 1 or q.shape[-1] == 1) and ld % 16 == 0 and ld >= q.shape[-1] and q.data_ptr() % 16 == 0
+    if q.dim() == 3 and q.shape[0] > 1:
+        ok = ok and q.stride(0) == ld * q.shape[1]
+    return ld if ok else None
+
+
+def fp8_table_stride(name, q, s, lead, rows, K, device):
+    """Checks one table of block-scaled codes (q [*lead, rows, K] as fp8_pad_rows leaves it, s its scales); its row
+    stride in bytes."""
+    want = (*lead, -(-rows // 128), -(-K // 128))
+    if q.dtype != torch.float8_e4m3fn or tuple(q.shape) != (*lead, rows, K):
+        raise ValueError(f"{name}: codes are float8_e4m3fn {(*lead, rows, K)}, got {q.dtype} {tuple(q.shape)}")
+    if s.dtype != torch.float32 or tuple(s.shape) != want or not s.is_contiguous():
+        raise ValueError(f"{name}: scales are contiguous fp32 {want}, got {s.dtype} {tuple(s.shape)}")
+    if q.device != device or s.device != device:
+        raise ValueError(f"{name}: tensors on {q.device} and {s.device}, expected {device}")
+    ld = fp8_row_stride(q)
+    if ld is None:
+        raise ValueError(f"{name}: rows are not 16-byte aligned at a stride of a multiple of 16: use fp8_pad_rows")
+    return ld
+
+
+def fp8_linear(q, s, x, out_dtype=torch.float32):
+    """x [N, K] @ W^T -> [N, rows] in out_dtype (fp32, bf16, fp16), W = e4m3 codes q [rows, K] (fp8_pad_rows) times fp32
+    scales s [ceil(rows / 128), ceil(K / 128)] of 128 x 128 blocks. x: bf16, fp16 or fp32, quantised per row in groups of
+    128 as fp8_quantize does, or the pair (codes, scales) that fp8_quantize returned (one quantisation for several
+    products). fp32 sums. Inference only: no gradient."""
+    ready = isinstance(x, (tuple, list))
+    xv, xs = x if ready else (x, None)
+    require_cuda(q, s, xv, xs)
+    if q.dim() != 2 or xv.dim() != 2 or xv.shape[1] != q.shape[1] or q.shape[0] == 0 or q.shape[1] == 0:
+        raise ValueError(f"q [rows, K] and x [N, K], got {tuple(q.shape)} and {tuple(xv.shape)}")
+    if out_dtype not in TYPES:
+        raise ValueError(f"out_dtype is fp32, bf16 or fp16, got {out_dtype}")
+    (rows, K), N = q.shape, xv.shape[0]
+    ldq = fp8_table_stride("weights", q, s, (), rows, K, xv.device)
+    if ready:
+        if xv.dtype != torch.float8_e4m3fn:
+            raise ValueError(f"a pair holds float8_e4m3fn codes, got {xv.dtype}")
+        if xs.dtype != torch.float32 or tuple(xs.shape) != (N, -(-K // 128)) or xs.device != xv.device:
+            raise ValueError(f"scales of x are fp32 {(N, -(-K // 128))} on {xv.device}, got {xs.dtype} {tuple(xs.shape)}")
+        xv, xs = fp8_pad_rows(xv), xs.contiguous()
+        ldx, code = (fp8_row_stride(xv) if N > 0 else K), E4M3
+    else:
+        if xv.dtype not in TYPES:
+            raise ValueError(f"x is bf16, fp16 or fp32, got {xv.dtype}")
+        xv, ldx = _fp8_x(xv)
+        code = TYPES[xv.dtype]
+    with torch.cuda.device(xv.device):
+        y = torch.empty((N, rows), dtype=out_dtype, device=xv.device)
+        nbytes = lib().cbmoe_fp8_linear_workspace_bytes(N, K, rows, code)
+        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=xv.device)
+        check(lib().cbmoe_fp8_linear(ptr(q), ldq, ptr(s), rows, K, ptr(xv), code, ldx, ptr(xs), N, ptr(y),
+                                     TYPES[out_dtype], ptr(ws), nbytes, stream_handle()), "cbmoe_fp8_linear")
+    return y

@@ -13,7 +13,7 @@ asserts; there is no CPU fallback.
 """
 import torch
 
-from . import iq, ops
+from . import fp8, iq, ops
 from ._lib import PATHS, Experts, Shared, check, lib, ptr, require_cuda, stream_handle
 
 CB3 = "CB3"
@@ -60,7 +60,7 @@ class ResidentFetch:
     """Stored on the engine; `apply(p, x, idx, w, layer, limit)` as in resident.py:100-108.
 
     Constructor knobs keep the reference's names: `qtypes` {layer: {"gate_q", "up_q", "down_q"} -> format}
-    ("CB3" only here), `D`, `ml` (this GPU's intermediate size), `out_dtype` of the returned partial,
+    ("CB3" only here; the GGUF formats of cbmoe.iq and "FP8" of cbmoe.fp8 by their tables), `D`, `ml` (this GPU's intermediate size), `out_dtype` of the returned partial,
     `gather_max_rows` (slots N*k at or below which the decode kernels run; above it the grouped path), and
     `path` to force "decode" or "grouped"."""
 
@@ -90,7 +90,7 @@ class ResidentFetch:
     def _check(self, p, x, idx, w, layer):
         require_cuda(x, idx, w)
         for key in ("gate_q", "up_q", "down_q"):
-            have = p["qtypes"][key] if p.get("format") == "IQ" else CB3
+            have = p["qtypes"][key] if p.get("format") in ("IQ", fp8.FP8) else CB3
             qt = self.qtypes.get(layer, {}).get(key, have)
             if qt != have:
                 raise ValueError(f"layer {layer} {key}: qtypes says {qt}, the tables hold {have}")
@@ -113,6 +113,8 @@ class ResidentFetch:
         xb = x.to(torch.bfloat16).contiguous()
         idx = idx.to(torch.int32).contiguous()
         w = w.to(torch.float32).contiguous()
+        if p.get("format") == fp8.FP8:   # e4m3 tables with 128 x 128 block scales (cbmoe.fp8.pack_layer)
+            return fp8.apply(p, xb, idx, w, limit, self.out_dtype)
         y = torch.empty((N, p["H"]), dtype=torch.float32, device=x.device)
         path = self._path_code(N, k)
         ex, ws = self.workspace(p, N, k, path, x.device)

@@ -392,17 +392,7 @@ done:
 
 // ------------------------------------------------------------------------------------------ tensor maps
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::mutex mu;
-  std::lock_guard<std::mutex> lk(mu);
-  if (fn == nullptr) {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q{};
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
-  }
-  return fn;
+  return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tensor_map_encoder());
 }
 
 // bf16 matrix [rows][K] (row stride K*2 bytes): 64 x 128 boxes, 128-byte swizzle, zero fill out of bounds.
@@ -527,6 +517,20 @@ int grid_of(long long total) {
 }
 
 }  // namespace
+
+void* tensor_map_encoder() {
+  static void* fn = nullptr;
+  static std::mutex mu;
+  std::lock_guard<std::mutex> lk(mu);
+  if (fn == nullptr) {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = ptr;
+  }
+  return fn;
+}
 
 int grouped_cb3_gateup(const GroupedParams& p, const void* b, int b_rows, int tn, cudaStream_t s) {
   if (tn == 128) return launch_grouped<kFmtCB3, 2, kGrpEpiSwiglu, 128>(p, b, b_rows, kProfGrpCb3GateUp, s);

@@ -34,6 +34,9 @@ struct GroupedParams {
   float* out_f32;          // kGrpEpiStoreF32
 };
 
+// The driver's cuTensorMapEncodeTiled (looked up once; null when it is missing).
+void* tensor_map_encoder();
+
 // tn: token rows per pass of the routing plan (128 or 256).
 int grouped_cb3_gateup(const GroupedParams& p, const void* b, int b_rows, int tn, cudaStream_t s);
 int grouped_cb3_down(const GroupedParams& p, const void* b, int b_rows, int tn, cudaStream_t s);

@@ -1,0 +1,299 @@
+// Tokens into expert order and back, forward and backward, over a routing plan (cbmoe_route_plan): the row gather and
+// the weighted combine of the layer (resident.py:144-165) as operators of their own, with their gradients.
+//
+//   permute             xs[r] = x[tok_row[r]], zero rows where tok_row[r] < 0
+//   unpermute           y[t] = sum_j w[t, j] ys[row_slot[t, j]]      (without w: the plain sum, permute's gradient)
+//   unpermute backward  dys[row_slot[t, j]] = w[t, j] dy[t], zero rows where tok_row < 0; dw[t, j] = <dy[t], ys[row]>
+//
+// All three are bound by memory, so each walks the tokens, not the sorted rows: a token's row is read once and its k
+// sorted rows are written (or read) once, and no row is touched twice. A sorted row belongs to one slot, so nothing is
+// added by atomics: sums run over j in order, in fp32, rounded once. Rows outside [0, R) in row_slot are empty slots.
+#include <cuda_fp16.h>
+
+#include "decode.cuh"
+#include "profile.cuh"
+
+namespace cbmoe {
+
+namespace {
+
+constexpr int kPermThreads = 256;
+
+template <typename T>
+struct Elem;
+template <>
+struct Elem<__nv_bfloat16> {
+  static __device__ float to(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static __device__ __nv_bfloat16 from(float v) { return __float2bfloat16_rn(v); }
+};
+template <>
+struct Elem<__half> {
+  static __device__ float to(__half v) { return __half2float(v); }
+  static __device__ __half from(float v) { return __float2half_rn(v); }
+};
+template <>
+struct Elem<float> {
+  static __device__ float to(float v) { return v; }
+  static __device__ float from(float v) { return v; }
+};
+
+// VB bytes of a row as one unit: 16 where rows and pointers are 16-byte aligned, else one element.
+template <typename T, int VB>
+struct alignas(VB) Vec {
+  static constexpr int n = VB / (int)sizeof(T);
+  T v[n];
+};
+
+// Zero rows of `out` where tok_row < 0: a warp looks at 32 rows at a time.
+template <typename V>
+__device__ __forceinline__ void zero_padding(V* out, const int32_t* __restrict__ tok_row, int R, int HV, int warp0,
+                                             int n_warps) {
+  const int lane = threadIdx.x & 31;
+  for (long long base = 32LL * warp0; base < R; base += 32LL * n_warps) {
+    const int r = (int)base + lane;
+    unsigned todo = __ballot_sync(0xffffffffu, r < R && tok_row[r < R ? r : R - 1] < 0);
+    while (todo) {
+      const int row = (int)base + __ffs(todo) - 1;
+      todo &= todo - 1;
+      V z{};
+      for (int c = lane; c < HV; c += 32) out[(size_t)row * HV + c] = z;
+    }
+  }
+}
+
+template <typename T, int VB>
+__global__ void __launch_bounds__(kPermThreads) permute_kernel(const Vec<T, VB>* __restrict__ x, int Tn, int HV,
+                                                               const int32_t* __restrict__ row_slot, int k,
+                                                               const int32_t* __restrict__ tok_row, int R,
+                                                               Vec<T, VB>* __restrict__ xs, int tok_blocks) {
+  griddep_wait();
+  griddep_launch();
+  if ((int)blockIdx.x >= tok_blocks) {
+    zero_padding(xs, tok_row, R, HV, ((int)blockIdx.x - tok_blocks) * (kPermThreads / 32) + (threadIdx.x >> 5),
+                 ((int)gridDim.x - tok_blocks) * (kPermThreads / 32));
+    return;
+  }
+  const long long total = (long long)Tn * HV;
+  for (long long i = blockIdx.x * (long long)kPermThreads + threadIdx.x; i < total;
+       i += (long long)tok_blocks * kPermThreads) {
+    const int t = (int)(i / HV), c = (int)(i - (long long)t * HV);
+    const Vec<T, VB> v = x[i];
+    for (int j = 0; j < k; ++j) {
+      const int r = row_slot[(size_t)t * k + j];
+      if (r >= 0 && r < R) xs[(size_t)r * HV + c] = v;
+    }
+  }
+}
+
+template <typename T, int VB>
+__global__ void __launch_bounds__(kPermThreads) unpermute_kernel(const Vec<T, VB>* __restrict__ ys, int R, int HV,
+                                                                 const int32_t* __restrict__ row_slot,
+                                                                 const float* __restrict__ w, int Tn, int k,
+                                                                 Vec<T, VB>* __restrict__ y) {
+  using V = Vec<T, VB>;
+  griddep_wait();
+  griddep_launch();
+  const long long total = (long long)Tn * HV;
+  for (long long i = blockIdx.x * (long long)kPermThreads + threadIdx.x; i < total;
+       i += (long long)gridDim.x * kPermThreads) {
+    const int t = (int)(i / HV), c = (int)(i - (long long)t * HV);
+    float acc[V::n] = {};
+    for (int j0 = 0; j0 < k; j0 += 8) {   // 8 rows in flight
+      V v[8];
+      float wt[8];
+      bool in[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int r = j0 + j < k ? row_slot[(size_t)t * k + j0 + j] : -1;
+        in[j] = r >= 0 && r < R;
+        wt[j] = in[j] && w != nullptr ? w[(size_t)t * k + j0 + j] : 1.f;
+        if (in[j]) v[j] = ys[(size_t)r * HV + c];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (in[j]) {
+#pragma unroll
+          for (int q = 0; q < V::n; ++q) acc[q] = fmaf(wt[j], Elem<T>::to(v[j].v[q]), acc[q]);
+        }
+    }
+    V o;
+#pragma unroll
+    for (int q = 0; q < V::n; ++q) o.v[q] = Elem<T>::from(acc[q]);
+    y[i] = o;
+  }
+}
+
+constexpr int kBackThreads = 128;
+
+// One CTA per token (grid-stride): dy[t] is read once per 8 slots, dw by a fixed-order block sum.
+template <typename T, int VB>
+__global__ void __launch_bounds__(kBackThreads) unpermute_backward_kernel(
+    const Vec<T, VB>* __restrict__ dy, const Vec<T, VB>* __restrict__ ys, int R, int HV,
+    const int32_t* __restrict__ row_slot, const int32_t* __restrict__ tok_row, const float* __restrict__ w, int Tn,
+    int k, Vec<T, VB>* __restrict__ dys, float* __restrict__ dw, int tok_blocks) {
+  using V = Vec<T, VB>;
+  __shared__ float red[8][kBackThreads / 32];
+  griddep_wait();
+  griddep_launch();
+  if ((int)blockIdx.x >= tok_blocks) {
+    zero_padding(dys, tok_row, R, HV, ((int)blockIdx.x - tok_blocks) * (kBackThreads / 32) + (threadIdx.x >> 5),
+                 ((int)gridDim.x - tok_blocks) * (kBackThreads / 32));
+    return;
+  }
+  for (int t = blockIdx.x; t < Tn; t += tok_blocks) {
+    for (int j0 = 0; j0 < k; j0 += 8) {
+      int r[8];
+      float wt[8], dot[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        r[j] = j0 + j < k ? row_slot[(size_t)t * k + j0 + j] : -1;
+        if (r[j] >= R) r[j] = -1;
+        wt[j] = r[j] >= 0 && w != nullptr ? w[(size_t)t * k + j0 + j] : 1.f;
+        dot[j] = 0.f;
+      }
+      for (int c = threadIdx.x; c < HV; c += kBackThreads) {
+        const V d = dy[(size_t)t * HV + c];
+        V v[8];
+        if (dw != nullptr) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (r[j] >= 0) v[j] = ys[(size_t)r[j] * HV + c];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (r[j] < 0) continue;
+          V o;
+#pragma unroll
+          for (int q = 0; q < V::n; ++q) {
+            const float g = Elem<T>::to(d.v[q]);
+            o.v[q] = Elem<T>::from(wt[j] * g);
+            if (dw != nullptr) dot[j] = fmaf(g, Elem<T>::to(v[j].v[q]), dot[j]);
+          }
+          if (dys != nullptr) dys[(size_t)r[j] * HV + c] = o;
+        }
+      }
+      if (dw == nullptr) continue;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+#pragma unroll
+        for (int m = 16; m > 0; m >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], m);
+        if ((threadIdx.x & 31) == 0) red[j][threadIdx.x >> 5] = dot[j];
+      }
+      __syncthreads();
+      if (threadIdx.x < 8 && j0 + (int)threadIdx.x < k) {
+        float s = 0.f;
+#pragma unroll
+        for (int u = 0; u < kBackThreads / 32; ++u) s += red[threadIdx.x][u];
+        dw[(size_t)t * k + j0 + threadIdx.x] = s;   // 0 for an empty slot
+      }
+      __syncthreads();
+    }
+  }
+}
+
+int blocks_for(long long total, int threads, int per_sm) {
+  const long long b = (total + threads - 1) / threads, cap = (long long)num_sms() * per_sm;
+  return (int)(b < 1 ? 1 : (b > cap ? cap : b));
+}
+
+// Blocks beside the token blocks that clear padding rows (each warp checks 32 rows at a time).
+int pad_blocks(int R, int threads) {
+  const long long b = ((long long)R + threads - 1) / threads, cap = num_sms();
+  return (int)(b > cap ? cap : b);
+}
+
+size_t elem_size(int type) { return type == CBMOE_F32 ? 4 : 2; }
+
+bool vec16(int type, int H, const void* a, const void* b, const void* c = nullptr) {
+  auto ok = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  return (size_t)H * elem_size(type) % 16 == 0 && ok(a) && ok(b) && ok(c);
+}
+
+template <typename T, int VB>
+int permute_t(const void* x, int Tn, int H, const int32_t* row_slot, int k, const int32_t* tok_row, int R, void* xs,
+              cudaStream_t s) {
+  using V = Vec<T, VB>;
+  const int HV = H / V::n, tb = blocks_for((long long)Tn * HV, kPermThreads, 32);
+  CBMOE_CUDA_TRY(launch_pdl(permute_kernel<T, VB>, dim3(tb + pad_blocks(R, kPermThreads)), dim3(kPermThreads), 0, s,
+                            static_cast<const V*>(x), Tn, HV, row_slot, k, tok_row, R, static_cast<V*>(xs), tb));
+  return CBMOE_OK;
+}
+
+template <typename T, int VB>
+int unpermute_t(const void* ys, int R, int H, const int32_t* row_slot, const float* w, int Tn, int k, void* y,
+                cudaStream_t s) {
+  using V = Vec<T, VB>;
+  const int HV = H / V::n;
+  CBMOE_CUDA_TRY(launch_pdl(unpermute_kernel<T, VB>, dim3(blocks_for((long long)Tn * HV, kPermThreads, 32)),
+                            dim3(kPermThreads), 0, s, static_cast<const V*>(ys), R, HV, row_slot, w, Tn, k,
+                            static_cast<V*>(y)));
+  return CBMOE_OK;
+}
+
+template <typename T, int VB>
+int unpermute_backward_t(const void* dy, const void* ys, int R, int H, const int32_t* row_slot, const int32_t* tok_row,
+                         const float* w, int Tn, int k, void* dys, float* dw, cudaStream_t s) {
+  using V = Vec<T, VB>;
+  const int HV = H / V::n, tb = blocks_for(Tn, 1, 64);
+  const int pb = dys != nullptr ? pad_blocks(R, kBackThreads) : 0;
+  CBMOE_CUDA_TRY(launch_pdl(unpermute_backward_kernel<T, VB>, dim3(tb + pb), dim3(kBackThreads), 0, s,
+                            static_cast<const V*>(dy), static_cast<const V*>(ys), R, HV, row_slot, tok_row, w, Tn, k,
+                            static_cast<V*>(dys), dw, tb));
+  return CBMOE_OK;
+}
+
+bool type_ok(int t) { return t == CBMOE_BF16 || t == CBMOE_F16 || t == CBMOE_F32; }
+
+}  // namespace
+
+// f<T, VB>(args...) for the type and for whole 16-byte units or single elements.
+#define CBMOE_BY_TYPE(f, type, wide, ...)                                                            \
+  ((type) == CBMOE_BF16  ? ((wide) ? f<__nv_bfloat16, 16>(__VA_ARGS__) : f<__nv_bfloat16, 2>(__VA_ARGS__)) \
+   : (type) == CBMOE_F16 ? ((wide) ? f<__half, 16>(__VA_ARGS__) : f<__half, 2>(__VA_ARGS__))          \
+                         : ((wide) ? f<float, 16>(__VA_ARGS__) : f<float, 4>(__VA_ARGS__)))
+
+}  // namespace cbmoe
+
+using namespace cbmoe;
+
+extern "C" int cbmoe_permute(const void* x, int type, int T, int H, const int32_t* row_slot, int k,
+                             const int32_t* tok_row, int R, void* xs, cudaStream_t stream) {
+  if (!type_ok(type) || T < 0 || H <= 0 || k <= 0 || R < 0) return CBMOE_ERR_INVALID;
+  if ((T > 0 && (!x || !row_slot)) || (R > 0 && (!tok_row || !xs))) return CBMOE_ERR_INVALID;
+  if (R == 0) return CBMOE_OK;
+  prof_begin(kProfOther, stream);
+  const int rc = CBMOE_BY_TYPE(permute_t, type, vec16(type, H, x, xs), x, T, H, row_slot, k, tok_row, R, xs, stream);
+  prof_end(kProfOther, stream);
+  if (rc) return rc;
+  CBMOE_CUDA_TRY(cudaGetLastError());
+  return CBMOE_OK;
+}
+
+extern "C" int cbmoe_unpermute(const void* ys, int type, int R, int H, const int32_t* row_slot, const float* w, int T,
+                               int k, void* y, cudaStream_t stream) {
+  if (!type_ok(type) || T < 0 || H <= 0 || k <= 0 || R < 0) return CBMOE_ERR_INVALID;
+  if (T > 0 && (!row_slot || !y || (R > 0 && !ys))) return CBMOE_ERR_INVALID;
+  if (T == 0) return CBMOE_OK;
+  prof_begin(kProfCombine, stream);
+  const int rc = CBMOE_BY_TYPE(unpermute_t, type, vec16(type, H, ys, y), ys, R, H, row_slot, w, T, k, y, stream);
+  prof_end(kProfCombine, stream);
+  if (rc) return rc;
+  CBMOE_CUDA_TRY(cudaGetLastError());
+  return CBMOE_OK;
+}
+
+extern "C" int cbmoe_unpermute_backward(const void* dy, const void* ys, int type, int R, int H,
+                                        const int32_t* row_slot, const int32_t* tok_row, const float* w, int T, int k,
+                                        void* dys, float* dw, cudaStream_t stream) {
+  if (!type_ok(type) || T < 0 || H <= 0 || k <= 0 || R < 0) return CBMOE_ERR_INVALID;
+  if ((T > 0 && (!dy || !row_slot)) || (dw && R > 0 && !ys) || (dys && R > 0 && !tok_row)) return CBMOE_ERR_INVALID;
+  if (!dys && !dw) return CBMOE_OK;
+  if (T == 0 && (!dys || R == 0)) return CBMOE_OK;
+  prof_begin(kProfCombine, stream);
+  const int rc = CBMOE_BY_TYPE(unpermute_backward_t, type, vec16(type, H, dy, dys, ys), dy, ys, R, H, row_slot,
+                               tok_row, w, T, k, dys, dw, stream);
+  prof_end(kProfCombine, stream);
+  if (rc) return rc;
+  CBMOE_CUDA_TRY(cudaGetLastError());
+  return CBMOE_OK;
+}
