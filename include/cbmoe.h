@@ -244,8 +244,8 @@ int cbmoe_fp8_quantize(const void* x, int type, int N, int K, long long ldx, uin
                        cudaStream_t stream);
 /* y [N][rows] (y_type) = x W^T, W = e4m3 codes q with scales s. x: bf16, fp16 or fp32 (quantised here, xs NULL), or
  * CBMOE_E4M3 codes with their scales xs [N][ceil(K/128)] as cbmoe_fp8_quantize makes them (any fp32 scales; ldx a
- * multiple of 16, x 16-byte aligned). fp32 sums. Workspace: the query (256-byte aligned; zero bytes for
- * CBMOE_E4M3 input below a size that needs partial sums). */
+ * multiple of 16, x 16-byte aligned). fp32 sums. Workspace: the query, 256-byte aligned (the
+ * quantised x, and partial sums of output tiles that several SMs share). */
 size_t cbmoe_fp8_linear_workspace_bytes(int N, int K, int rows, int x_type);
 int cbmoe_fp8_linear(const void* q, long long ldq, const float* s, int rows, int K, const void* x, int x_type,
                      long long ldx, const float* xs, int N, void* y, int y_type, void* workspace,

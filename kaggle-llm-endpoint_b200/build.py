@@ -3,7 +3,7 @@
     python kaggle-llm-endpoint_b200/build.py          # -> kaggle-llm-endpoint_b200/cbmoe/libcbmoe.so
 
 Every .cu under csrc/ is compiled with relocatable device code (one device symbol, the error word, is shared
-across files) and linked into one shared library with the CUDA runtime linked statically. Objects go to
+across files; OWN_UNIT below names the exceptions) and linked into one shared library with the CUDA runtime linked statically. Objects go to
 _build/ next to this file; a file is recompiled when it or any header under csrc/ or include/ is newer.
 """
 import glob
@@ -19,6 +19,9 @@ INCLUDE = os.path.join(ROOT, "include")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "cbmoe", "libcbmoe.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
+# Compiled without relocatable device code: their kernels move registers between warpgroups (setmaxnreg), which ptxas
+# ignores in relocatable code. Such a file shares no device symbol with the others (common.cuh).
+OWN_UNIT = {"fp8.cu"}
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ARCH + ["-O3", "-lineinfo", "-std=c++17", "-rdc=true", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
                 "-I", INCLUDE, "-I", CSRC]
@@ -33,7 +36,8 @@ def _compile(src, extra, verbose):
     obj = os.path.join(BUILD, os.path.basename(src).replace(".cu", ".o"))
     if os.path.exists(obj) and os.path.getmtime(obj) >= max(os.path.getmtime(src), _newest_header()):
         return obj
-    cmd = [NVCC] + FLAGS + extra + ["-c", src, "-o", obj]
+    flags = [f for f in FLAGS if f != "-rdc=true"] if os.path.basename(src) in OWN_UNIT else FLAGS
+    cmd = [NVCC] + flags + extra + ["-c", src, "-o", obj]
     if verbose:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)

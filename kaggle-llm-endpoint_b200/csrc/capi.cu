@@ -5,6 +5,7 @@
 #include <mutex>
 
 #include "decode.cuh"
+#include "fp8.cuh"
 #include "grouped.cuh"
 #include "layer.cuh"
 
@@ -514,7 +515,10 @@ extern "C" int cbmoe_device_errors(int clear, int* out_host) {
   CBMOE_CUDA_TRY(cudaDeviceSynchronize());
   int v = 0;
   CBMOE_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_device_errors, sizeof(int)));
-  *out_host = v;
+  int fp8 = 0;
+  const int rc = fp8_device_errors(clear, &fp8);
+  if (rc) return rc;
+  *out_host = v | fp8;
   if (clear) {
     const int zero = 0;
     CBMOE_CUDA_TRY(cudaMemcpyToSymbol(g_device_errors, &zero, sizeof(int)));

@@ -12,7 +12,13 @@ namespace cbmoe {
 
 // Device-side error word. Kernels OR a CBMOE_DEVERR_* bit into it instead of trapping; the host reads it with
 // cbmoe_device_errors(). It is an error flag, not scratch: kernels never read it back.
+// A file compiled without relocatable device code (build.py: setmaxnreg needs a kernel whose registers are known when
+// it is compiled) defines CBMOE_OWN_UNIT and has a word of its own, which cbmoe_device_errors() reads too.
+#ifdef CBMOE_OWN_UNIT
+static __device__ int g_device_errors = 0;
+#else
 extern __device__ int g_device_errors;
+#endif
 
 constexpr unsigned long long kWaitLimitNs = 4000000000ull;   // 4 s: every spin-wait gives up after this
 
@@ -69,6 +75,39 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
     }
   }
   return true;
+}
+
+// Arrive on the barrier at the same shared-memory offset of CTA `rank` of the cluster. Orders no ordinary memory accesses
+// between the CTAs: it tells of finished TMA loads and TMEM reads only.
+__device__ __forceinline__ void mbar_arrive_remote(uint64_t* bar, uint32_t rank) {
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\t"
+      "mapa.shared::cluster.u32 a, %0, %1;\n\t"
+      "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}\n" ::"r"(smem_addr(bar)),
+      "r"(rank)
+      : "memory");
+}
+
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(p));
+  return p != 0;
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+// All threads of the cluster's CTAs (each CTA reaches it: every wait before it is bounded).
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
 // The same wait for a warp that is usually early (a producer waiting for consumers to free a stage): it sleeps

@@ -2,19 +2,29 @@
 //
 //   y[n, r] = sum_b sx[n, b] * sw[r / 128, b] * sum_{c in block b} xq[n, c] * wq[r, c]
 //
-// fp8_gemm_kernel, one CTA per SM, 10 warps:
-//   warp 0     TMA producer: per 128-column block the tile's MT x 128 B of tokens and 2 x 128 x 128 B of weights (128-byte
-//              swizzle), into a ring of stages
-//   warp 1     TMEM owner and MMA issuer (one thread): 4 tcgen05.mma kind::f8f6f4 (M 128 x N 256 x K 32) per block into
-//              one of two 256-column accumulators
-//   warps 2-9  promotion and epilogue: a block's 128 x 256 partial sums leave TMEM while the tensor core works on the next
-//              block; acc += partial * (sx * sw) in fp32 registers (32 rows x 128 columns per warp). Tokens are the M side,
-//              so a thread owns one token row: both scales are scalars for its columns.
+// fp8_gemm_kernel, one CTA per SM, 12 warps:
+//   warp 0      TMA producer: per 128-column block the tile's MT x 128 B of tokens and 2 x 128 x 128 B of weights (128-byte
+//               swizzle), into a ring of stages
+//   warp 1      TMEM owner and MMA issuer (one thread): 4 tcgen05.mma kind::f8f6f4 (M 128 x N 256 x K 32) per block into
+//               one of two 256-column accumulators
+//   warps 4-11  promotion and epilogue: a block's 128 x 256 partial sums leave TMEM while the tensor core works on the next
+//               block; acc += partial * (sx * sw) in fp32 registers (32 rows x 128 columns per warp). Tokens are the M side,
+//               so a thread owns one token row: both scales are scalars for its columns. These warps take the registers
+//               that the first warpgroup gives up (128 accumulators + two 32-column loads in turn a thread).
 // The block's partial sum is exact enough to be added as it is: e4m3 products are exact in fp32 and the tensor core sums
 // them in fp32 (measured: 1e-8 relative over K = 128).
+// With many rows (MT = 256) two CTAs of a cluster work as a pair (cta_group::2, M = 256): each brings 128 tokens and half
+// of the weight tile, so a block costs an SM 32 KB of shared-memory writes and 32 KB of operand reads where a CTA alone
+// costs it 48 and 48, which at 128 B a clock is more than the 512 clocks of its MMAs (measured at 4096 x 5120 x 12288:
+// alone 1300 clocks a block, 1070 with the promotion left out).
 // With two matrices (gate, up: 128 columns each) the epilogue forms swiglu_clamped(gate, up), takes each row's maximum
 // over its 128 columns and stores e4m3 codes and the scale: the down product's input, never in 16 bits.
+// Work: whole waves of output tiles, one tile per CTA; the tiles left over are cut along K into equal ranges of blocks, one
+// per CTA (Fp8Sched), so that few rows (a single token: all of the time) still use every SM and the memory behind it. A
+// tile's ranges leave fp32 partial sums in the workspace; the last to arrive adds them in range order (the same bits on
+// every call) and runs the epilogue.
 // Every wait is bounded; a role that gives up sets CBMOE_DEVERR_TIMEOUT and falls through to the final barrier.
+#define CBMOE_OWN_UNIT
 #include <cudaTypedefs.h>
 
 #include "fp8.cuh"
@@ -42,10 +52,11 @@ __device__ __forceinline__ float to_f32(float v) { return v; }
 template <typename T>
 __global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__ x, int N, int K, long long ldx,
                                                            int vec, uint8_t* __restrict__ q, long long ldq,
-                                                           float* __restrict__ s, const int* __restrict__ row_slot,
-                                                           int k, int R) {
+                                                           float* __restrict__ s, int lds,
+                                                           const int* __restrict__ row_slot, int k, int R, int* __restrict__ zero, int n_zero) {
   griddep_wait();
   griddep_launch();
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < n_zero; i += gridDim.x * 256) zero[i] = 0;
   const int KB = (K + kFp8Group - 1) / kFp8Group;
   const long long total = (long long)N * KB;
   const int l = threadIdx.x & 15;
@@ -90,29 +101,36 @@ __global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__
       } else {
         for (int i = 0; i < 8 && c0 + i < K; ++i) dst[i] = (uint8_t)((i < 4 ? o.x : o.y) >> (8 * (i & 3)));
       }
-      if (l == 0) s[(size_t)r * KB + kb] = sc;
+      if (l == 0) s[(size_t)r * lds + kb] = sc;
     }
   }
 }
 
 // --------------------------------------------------------------------------------------------------- product
-constexpr int kFp8Threads = 10 * 32;
-constexpr int kW0 = 2;                                   // first promotion warp
+constexpr int kFp8Threads = 12 * 32;
+constexpr int kW0 = 4;                                   // first promotion warp
 constexpr int kBHalf = 128 * 128;                        // 128 weight rows of one block
+constexpr int kRegsIdle = 40, kRegsWork = 232;           // 128 * 40 + 256 * 232 = 384 * 168, the launch's registers
 
 template <int MT>
 struct Fp8Cfg {
-  static constexpr int kATile = MT * 128;
-  static constexpr int kStage = kATile + 2 * kBHalf;
-  static constexpr int kNStage = MT == 128 ? 4 : (MT == 64 ? 5 : 6);
+  static constexpr bool kPair = MT == 256;               // two CTAs, 128 tokens each
+  static constexpr int kRows = kPair ? 128 : MT;         // tokens of a CTA's tile
+  static constexpr int kATile = kRows * 128;
+  static constexpr int kStage = kATile + (kPair ? 1 : 2) * kBHalf;
+  static constexpr int kNStage = kPair ? 6 : (MT == 128 ? 4 : (MT == 64 ? 5 : 6));
   static constexpr int kBarOff = kNStage * kStage;
-  static constexpr int kSmem = 1024 + kBarOff + 256 + 4 * 2 * 2 * 32 * 4;   // + row maxima of the SwiGLU epilogue
+  static constexpr int kMaxOff = kBarOff + 256;          // row maxima [2][4 quadrants][2 halves][32] f32
+  static constexpr int kFlagOff = kMaxOff + 2048;        // [2][4] int
+  static constexpr int kSmem = 1024 + kFlagOff + 32;
   static_assert(kSmem <= 227 * 1024, "shared memory budget");
 };
 
 struct Fp8Params {
   Fp8Gemm g;
   int KB, RB, NT;          // column blocks, 128-row blocks per matrix, output tiles per pass
+  int hs_ld;               // row stride of hs
+  int xs_wide;             // xs rows are 16-byte aligned
 };
 
 struct Fp8Item {
@@ -131,23 +149,43 @@ __device__ __forceinline__ Fp8Item fp8_item(const Fp8Params& p, int item) {
   return {p.g.pass_expert[pass], p.g.pass_row0[pass], p.g.pass_cnt[pass], nt};
 }
 
-__device__ __forceinline__ void fma2(unsigned long long& acc, uint32_t lo, uint32_t hi, unsigned long long sc) {
-  unsigned long long d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
-  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(d), "l"(sc));
-}
+// A worker's (a CTA's, or a pair's) share of the tiles, in segments (tile, blocks [kb0, kb1)).
+struct Fp8Seg {
+  int item, kb0, kb1;
+};
+struct Fp8Sched {
+  int waves, first, KB, chunk, u, u1, i, worker, G;
 
-__device__ __forceinline__ unsigned long long pair_of(float v) {
-  unsigned long long d;
-  asm("mov.b64 %0, {%1, %1};" : "=l"(d) : "r"(__float_as_uint(v)));
-  return d;
-}
-
-__device__ __forceinline__ float lo_of(unsigned long long v) { return __uint_as_float((uint32_t)v); }
-__device__ __forceinline__ float hi_of(unsigned long long v) { return __uint_as_float((uint32_t)(v >> 32)); }
-
-// Accumulator pair i (columns 2i, 2i + 1) of a thread's 128 columns.
-#define CBMOE_ACC(a, c) (((c) & 1) ? hi_of((a)[(c) >> 1]) : lo_of((a)[(c) >> 1]))
+  // Ranges shorter than 4 blocks would spend more on joining them than on their sums.
+  // Worker `w` of `G` (a CTA, or a pair).
+  __device__ __forceinline__ Fp8Sched(int n_items, int kb, int w, int g) : KB(kb), i(0), worker(w), G(g) {
+    const int rem = n_items % G;
+    waves = n_items / G;
+    first = waves * G;
+    chunk = max((rem * KB + G - 1) / G, min(KB, 4));
+    u = min(rem * KB, worker * chunk);
+    u1 = min(rem * KB, u + chunk);
+  }
+  __device__ __forceinline__ bool next(Fp8Seg& s) {
+    if (i < waves) {
+      s = {i * G + worker, 0, KB};
+      ++i;
+      return true;
+    }
+    if (u >= u1) return false;
+    const int t = u / KB, kb0 = u - t * KB, kb1 = min(KB, kb0 + u1 - u);
+    s = {first + t, kb0, kb1};
+    u += kb1 - kb0;
+    return true;
+  }
+  // The workers [c0, c1] that share a left-over tile, and where a worker's partial sums of it lie.
+  __device__ __forceinline__ void sharers(int item, int& c0, int& c1) const {
+    const int b = (item - first) * KB;
+    c0 = b / chunk;
+    c1 = (b + KB - 1) / chunk;
+  }
+  __device__ __forceinline__ int slot(int w, int item) const { return 2 * w + (w * chunk / KB == item - first ? 0 : 1); }
+};
 
 template <typename OUT>
 __device__ __forceinline__ OUT out_of(float v);
@@ -158,11 +196,24 @@ __device__ __forceinline__ __nv_bfloat16 out_of(float v) { return __float2bfloat
 template <>
 __device__ __forceinline__ __half out_of(float v) { return __float2half_rn(v); }
 
+__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
 // silu(min(g, L)) * clip(u, -L, L) (model.py:119-122) that keeps a NaN, so that a bad row shows.
 __device__ __forceinline__ float swiglu_keep_nan(float g, float u, float limit) {
   g = g > limit ? limit : g;
   u = u > limit ? limit : (u < -limit ? -limit : u);
   return silu_f(g) * u;
+}
+
+// The two warps of a row quadrant wait for one another (bounded); `n` counts their meetings.
+__device__ __forceinline__ bool pair_meet(uint64_t* bar, uint32_t& n) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+  return mbar_wait(bar, n++ & 1);
 }
 
 template <int MT, bool SWIGLU, typename OUT>
@@ -177,24 +228,30 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const Fp8Param
   uint64_t* empty = full + C::kNStage;
   uint64_t* d_full = empty + C::kNStage;    // [2]
   uint64_t* d_empty = d_full + 2;           // [2]
-  uint64_t* swap = d_empty + 2;             // [4]: the two warps of a row quadrant exchange row maxima
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(swap + 4);
-  float* row_max = reinterpret_cast<float*>(smem + C::kBarOff + 256);   // [2 items][4 quadrants][2 halves][32]
+  uint64_t* meet = d_empty + 2;             // [4]
+  uint64_t* peer = meet + 4;                // [kNStage] pair, in rank 0: the other CTA's stage is full
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(peer + C::kNStage);
+  float* row_max = reinterpret_cast<float*>(smem + C::kMaxOff);
+  volatile int* flag = reinterpret_cast<volatile int*>(smem + C::kFlagOff);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kNStage; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
+      mbar_init(&peer[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&d_full[i], 1);
-      mbar_init(&d_empty[i], 8);
+      mbar_init(&d_empty[i], C::kPair ? 16 : 8);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(&swap[i], 2);
+    for (int i = 0; i < 4; ++i) mbar_init(&meet[i], 2);
     fence_mbar_init();
   }
-  if (warp == 1) tmem_alloc(tmem_slot, 512);
+  if (warp == 1) {
+    if constexpr (C::kPair) tmem_alloc_pair(tmem_slot, 512);
+    else tmem_alloc(tmem_slot, 512);
+  }
   if (warp == 0 && lane == 0) {
     prefetch_tmap(&map_x);
     prefetch_tmap(&map_w0);
@@ -202,68 +259,114 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const Fp8Param
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (C::kPair) cluster_sync();    // the other CTA's barriers are set up
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  const int rank = C::kPair ? (int)cluster_rank() : 0, group = C::kPair ? 2 : 1;
   griddep_wait();
   griddep_launch();
-  const int n_items = fp8_items<MT>(p);
 
-  if (warp == 0) {
-    if (lane == 0) {
-      int st = 0;
-      uint32_t ph = 0;
-      for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
-        const Fp8Item it = fp8_item<MT>(p, item);
-        const int wrow = it.e * p.g.rows + it.nt * (SWIGLU ? 128 : 256);
-        for (int kb = 0; kb < p.KB; ++kb) {
-          if (!mbar_wait_sleepy(&empty[st], ph ^ 1)) goto done;
+  if (warp < kW0) {
+    regs_give_up<kRegsIdle>();
+    Fp8Sched sched(fp8_items<MT>(p), p.KB, blockIdx.x / group, gridDim.x / group);
+    Fp8Seg sg;
+    // Whole warps walk these loops and one elected lane issues: addresses and descriptors stay in uniform registers, which
+    // halves the instructions of an issue (measured beside the promotion warps: 870 -> 760 clocks a block).
+    int st = 0;
+    uint32_t ph = 0;
+    if (warp == 0) {
+      while (sched.next(sg)) {
+        const Fp8Item it = fp8_item<MT>(p, sg.item);
+        const int wrow = it.e * p.g.rows + it.nt * (SWIGLU ? 128 : 256), xrow = it.row0 + 128 * rank;
+#pragma unroll 1
+        for (int kb = sg.kb0; kb < sg.kb1; ++kb) {
+          if (!mbar_wait(&empty[st], ph ^ 1)) goto done;
           uint8_t* a = smem + st * C::kStage;
-          mbar_arrive_expect_tx(&full[st], C::kStage);
-          tma_load_2d(a, &map_x, kb * kFp8Group, it.row0, &full[st]);
-          tma_load_2d(a + C::kATile, &map_w0, kb * kFp8Group, wrow, &full[st]);
-          tma_load_2d(a + C::kATile + kBHalf, SWIGLU ? &map_w1 : &map_w0, kb * kFp8Group, SWIGLU ? wrow : wrow + 128,
-                      &full[st]);
+          if (elect_one()) {
+            mbar_arrive_expect_tx(&full[st], C::kStage);
+            tma_load_2d(a, &map_x, kb * kFp8Group, xrow, &full[st]);
+            if (!C::kPair || rank == 0) tma_load_2d(a + C::kATile, &map_w0, kb * kFp8Group, wrow, &full[st]);
+            if (!C::kPair || rank == 1)
+              tma_load_2d(a + C::kATile + (C::kPair ? 0 : kBHalf), SWIGLU ? &map_w1 : &map_w0, kb * kFp8Group,
+                          SWIGLU ? wrow : wrow + 128, &full[st]);
+          }
+          __syncwarp();
           if (++st == C::kNStage) {
             st = 0;
             ph ^= 1;
           }
         }
       }
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = idesc_e4m3_m128(kFp8TileN);
-      int st = 0;
-      uint32_t ph = 0, n = 0;
-      for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
-        for (int kb = 0; kb < p.KB; ++kb, ++n) {
-          const int buf = n & 1;
-          if (!mbar_wait(&d_empty[buf], ((n >> 1) & 1) ^ 1) || !mbar_wait(&full[st], ph)) goto done;
-          tc_fence_after();
-          // Rows MT.. of the M side are whatever follows in the stage (weights): their sums are never read.
-          const uint32_t sbase = smem_addr(smem + st * C::kStage);
-          const uint64_t ad = sw128_desc(sbase), bd = sw128_desc(sbase + C::kATile);
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk) umma_fp8(tmem + buf * kFp8TileN, ad + 2 * kk, bd + 2 * kk, idesc, kk != 0);
-          umma_commit(&empty[st]);
-          umma_commit(&d_full[buf]);
+    } else if (warp == 1 && rank == 1) {
+      // The pair's MMAs are issued by rank 0: tell it which of this CTA's stages are full.
+      while (sched.next(sg)) {
+#pragma unroll 1
+        for (int kb = sg.kb0; kb < sg.kb1; ++kb) {
+          if (!mbar_wait(&full[st], ph)) goto done;
+          if (elect_one()) mbar_arrive_remote(&peer[st], 0);
+          __syncwarp();
           if (++st == C::kNStage) {
             st = 0;
             ph ^= 1;
           }
+        }
+      }
+    } else if (warp == 1) {
+      constexpr uint32_t idesc = idesc_e4m3(C::kPair ? 256 : 128, kFp8TileN);
+      const uint64_t desc0 = sw128_desc(smem_addr(smem));
+      uint32_t buf = 0, dph = 1;
+      while (sched.next(sg)) {
+#pragma unroll 1
+        for (int kb = sg.kb0; kb < sg.kb1; ++kb) {
+          if (!mbar_wait(&d_empty[buf], dph) || !mbar_wait(&full[st], ph)) goto done;
+          if (C::kPair && !mbar_wait(&peer[st], ph)) goto done;
+          tc_fence_after();
+          // Rows kRows.. of the M side are whatever follows in the stage (weights): their sums are never read.
+          const uint64_t ad = desc0 + (uint32_t)st * (C::kStage >> 4), bd = ad + (C::kATile >> 4);
+          const uint32_t d = tmem + buf * kFp8TileN;
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {
+              if constexpr (C::kPair) umma_fp8_pair(d, ad + 2 * kk, bd + 2 * kk, idesc, kk != 0);
+              else umma_fp8(d, ad + 2 * kk, bd + 2 * kk, idesc, kk != 0);
+            }
+            if constexpr (C::kPair) {
+              umma_commit_pair(&empty[st]);
+              umma_commit_pair(&d_full[buf]);
+            } else {
+              umma_commit(&empty[st]);
+              umma_commit(&d_full[buf]);
+            }
+          }
+          __syncwarp();
+          if (++st == C::kNStage) {
+            st = 0;
+            ph ^= 1;
+          }
+          buf ^= 1;
+          dph ^= buf ^ 1;
         }
       }
     }
   } else {
+    regs_take<kRegsWork>();
+    Fp8Sched sched(fp8_items<MT>(p), p.KB, blockIdx.x / group, gridDim.x / group);
+    Fp8Seg sg;
     const int q = warp & 3;                  // TMEM lane quadrant this warp may read
     const int half = (warp - kW0) >> 2;
-    uint32_t n = 0, local = 0;
-    for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
-      const Fp8Item it = fp8_item<MT>(p, item);
+    uint32_t n = 0, met = 0;
+    auto d_read = [&](int buf) {             // to the CTA that issues the MMAs
+      if (rank == 0) mbar_arrive(&d_empty[buf]);
+      else mbar_arrive_remote(&d_empty[buf], 0);
+    };
+    while (sched.next(sg)) {
+      Fp8Item it = fp8_item<MT>(p, sg.item);
+      it.row0 += 128 * rank;                 // this CTA's rows of the tile
+      it.cnt -= 128 * rank;
       const int m = 32 * q + lane;
       const bool live = 32 * q < it.cnt, mine = m < it.cnt;
-      const size_t xrow = (size_t)it.row0 + (mine ? m : 0);
-      const float* sx = p.g.xs + xrow * p.KB;
+      const size_t xrow = mine ? (size_t)it.row0 + m : 0;
+      const float* sx = p.g.xs + xrow * p.g.ldxs;
       const float *sa, *sb;                  // scales of this thread's columns 0-63 and 64-127
       if constexpr (SWIGLU) {
         sa = p.g.s0 + ((size_t)it.e * p.RB + it.nt) * p.KB;
@@ -272,99 +375,248 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const Fp8Param
         sa = p.g.s0 + ((size_t)it.e * p.RB + min(2 * it.nt + half, p.RB - 1)) * p.KB;
         sb = sa;
       }
-      unsigned long long acc[64];
+      float acc[128];
 #pragma unroll
-      for (int i = 0; i < 64; ++i) acc[i] = 0;
-      float x_next = live ? sx[0] : 0.f, a_next = sa[0], b_next = sb[0];
-      for (int kb = 0; kb < p.KB; ++kb, ++n) {
-        const int buf = n & 1;
-        const unsigned long long fa = pair_of(x_next * a_next), fb = pair_of(x_next * b_next);
-        if (live && kb + 1 < p.KB) {
-          x_next = sx[kb + 1];
-          a_next = sa[kb + 1];
-          if constexpr (SWIGLU) b_next = sb[kb + 1];
-          else b_next = a_next;
+      for (int i = 0; i < 128; ++i) acc[i] = 0.f;
+      // Scales come four blocks ahead of their use (a load's latency under the tiles' traffic is longer than a block):
+      // this row's own, four blocks at a time; the weights', one block per lane.
+      auto row_scales = [&](int kb) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p.xs_wide && kb % 4 == 0) {
+          if (kb < sg.kb1) v = *reinterpret_cast<const float4*>(sx + kb);
+        } else {
+          if (kb < sg.kb1) v.x = sx[kb];
+          if (kb + 1 < sg.kb1) v.y = sx[kb + 1];
+          if (kb + 2 < sg.kb1) v.z = sx[kb + 2];
+          if (kb + 3 < sg.kb1) v.w = sx[kb + 3];
         }
+        return v;
+      };
+      float4 xn = row_scales(sg.kb0), xc = xn;
+      float wa = 0.f, wb = 0.f, wa_n = 0.f, wb_n = 0.f;
+      if (sg.kb0 + lane < sg.kb1) {
+        wa_n = sa[sg.kb0 + lane];
+        if constexpr (SWIGLU) wb_n = sb[sg.kb0 + lane];
+      }
+      // Not unrolled: 128 multiply-adds a turn fill the instruction cache that the MMA issuer shares.
+#pragma unroll 1
+      for (int kb = sg.kb0; kb < sg.kb1; ++kb) {
+        const int at = kb - sg.kb0;
+        if (at % 4 == 0) {
+          xc = xn;
+          xn = row_scales(kb + 4);
+        }
+        if (at % 32 == 0) {
+          wa = wa_n, wb = wb_n;
+          if (kb + 32 + lane < sg.kb1) {
+            wa_n = sa[kb + 32 + lane];
+            if constexpr (SWIGLU) wb_n = sb[kb + 32 + lane];
+          }
+        }
+        const int buf = n & 1;
+        const float fa = xc.x * __shfl_sync(0xffffffffu, wa, at);
+        const float fb = SWIGLU ? xc.x * __shfl_sync(0xffffffffu, wb, at) : fa;
+        xc.x = xc.y, xc.y = xc.z, xc.z = xc.w;
         if (!mbar_wait(&d_full[buf], (n >> 1) & 1)) goto done;
+        ++n;
         tc_fence_after();
         if (live) {
           const uint32_t t0 = tmem + buf * kFp8TileN + ((uint32_t)(32 * q) << 16);
+          // 16 columns at a time: the two warps of a scheduler take turns between a load and its multiply-adds, and
+          // 128 + 16 registers a thread leave nothing to spill (loads of 32 columns or two in flight measured the same
+          // in a loop of their own, 350-370 clocks a block, and spilled here).
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t v[32];
-            const int col = SWIGLU ? (c < 2 ? 64 * half + 32 * c : 128 + 64 * half + 32 * (c - 2)) : 128 * half + 32 * c;
-            tmem_ld32(t0 + col, v);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) fma2(acc[16 * c + i], v[2 * i], v[2 * i + 1], c < 2 ? fa : fb);
-          }
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&d_empty[buf]);
-      }
-      if constexpr (SWIGLU) {
-        const int col0 = it.nt * 128 + 64 * half;
-        float top = 0.f;
-#pragma unroll
-        for (int i = 0; i < 64; ++i) {
-          const float h = col0 + i < p.g.rows ? swiglu_keep_nan(CBMOE_ACC(acc, i), CBMOE_ACC(acc, 64 + i), p.g.limit) : 0.f;
-          top = max_nan(top, fabsf(h));
-          if (i & 1) acc[i >> 1] = (acc[i >> 1] & 0xffffffffull) | ((unsigned long long)__float_as_uint(h) << 32);
-          else acc[i >> 1] = (acc[i >> 1] & ~0xffffffffull) | __float_as_uint(h);
-        }
-        float* mx = row_max + ((local & 1) * 4 + q) * 64;
-        mx[half * 32 + lane] = top;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&swap[q]);
-        if (!mbar_wait(&swap[q], local & 1)) goto done;
-        top = max_nan(top, mx[(half ^ 1) * 32 + lane]);
-        float inv;
-        const float sc = fp8_group_scale(top, &inv);
-        if (mine) {
-          uint4* dst = reinterpret_cast<uint4*>(p.g.hq + xrow * ((size_t)p.RB * 128) + col0);
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int c = 16 * u + 4 * i;
-              w[i] = fp8_pack4(CBMOE_ACC(acc, c) * inv, CBMOE_ACC(acc, c + 1) * inv, CBMOE_ACC(acc, c + 2) * inv,
-                               CBMOE_ACC(acc, c + 3) * inv);
+          for (int c = 0; c < 8; ++c) {       // 0-3 gate and 4-7 up; or 8 in a row
+            float v[16];
+            tmem_ld16(t0 + (SWIGLU ? (c < 4 ? 64 * half + 16 * c : 64 + 64 * half + 16 * c) : 128 * half + 16 * c), v);
+            if (c == 7) {                     // all of this block is in registers
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) d_read(buf);
             }
-            dst[u] = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[16 * c + i] = fmaf(v[i], c < 4 ? fa : fb, acc[16 * c + i]);
           }
-          if (half == 0) p.g.hs[xrow * p.RB + it.nt] = sc;
+        } else if (lane == 0) {
+          d_read(buf);
         }
-      } else if (mine) {
-        const int col0 = it.nt * 256 + 128 * half, rows = p.g.rows;
-        OUT* dst = static_cast<OUT*>(p.g.out) + xrow * rows + col0;
-        constexpr int kU = 16 / (int)sizeof(OUT);
-        if (rows % kU == 0 && (reinterpret_cast<uintptr_t>(p.g.out) & 15) == 0) {
+      }
+      const int rows = p.g.rows;
+      if (sg.kb0 == 0 && sg.kb1 == p.KB) {
+        // ------------------------------------------------------------- the whole sum: this thread's row, 128 columns
+        if constexpr (SWIGLU) {
+          const int col0 = it.nt * 128 + 64 * half;
+          float top = 0.f;
 #pragma unroll
-          for (int u = 0; u < 128 / kU; ++u) {
-            union {
-              uint4 v;
-              OUT o[kU];
-            } b;
+          for (int i = 0; i < 32; ++i) {
+            float h[2];
 #pragma unroll
-            for (int i = 0; i < kU; ++i) b.o[i] = out_of<OUT>(CBMOE_ACC(acc, u * kU + i));
-            if (col0 + u * kU < rows) reinterpret_cast<uint4*>(dst)[u] = b.v;
+            for (int c = 0; c < 2; ++c) {
+              h[c] = col0 + 2 * i + c < rows
+                         ? swiglu_keep_nan(acc[2 * i + c], acc[64 + 2 * i + c], p.g.limit)
+                         : 0.f;
+              top = max_nan(top, fabsf(h[c]));
+            }
+            acc[2 * i] = h[0];
+            acc[2 * i + 1] = h[1];
+          }
+          float* mx = row_max + ((met & 1) * 4 + q) * 64;
+          mx[half * 32 + lane] = top;
+          if (!pair_meet(&meet[q], met)) goto done;
+          top = max_nan(top, mx[(half ^ 1) * 32 + lane]);
+          float inv;
+          const float sc = fp8_group_scale(top, &inv);
+          if (mine) {
+            uint4* dst = reinterpret_cast<uint4*>(p.g.hq + xrow * ((size_t)p.RB * 128) + col0);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              uint32_t w[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int c = 16 * u + 4 * i;
+                w[i] = fp8_pack4(acc[c] * inv, acc[c + 1] * inv, acc[c + 2] * inv,
+                                 acc[c + 3] * inv);
+              }
+              dst[u] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            if (half == 0) p.g.hs[xrow * p.hs_ld + it.nt] = sc;
+          }
+        } else if (mine) {
+          const int col0 = it.nt * 256 + 128 * half;
+          OUT* dst = static_cast<OUT*>(p.g.out) + xrow * rows + col0;
+          constexpr int kU = 32 / (int)sizeof(OUT);        // one 32-byte store: a whole sector of this row
+          if (rows % kU == 0 && (reinterpret_cast<uintptr_t>(p.g.out) & 31) == 0) {
+#pragma unroll
+            for (int u = 0; u < 128 / kU; ++u) {
+              union {
+                uint32_t w[8];
+                OUT o[kU];
+              } b;
+#pragma unroll
+              for (int i = 0; i < kU; ++i) b.o[i] = out_of<OUT>(acc[u * kU + i]);
+              if (col0 + u * kU < rows) store32(dst + u * kU, b.w);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 128; ++i)
+              if (col0 + i < rows) dst[i] = out_of<OUT>(acc[i]);
+          }
+        }
+        continue;
+      }
+      // ----------------------------------------------- a range of the sum: partial sums [slot][rank][half][row][128 columns]
+      int c0, c1;
+      sched.sharers(sg.item, c0, c1);
+      auto part = [&](int w, int row) {
+        const size_t at = ((size_t)sched.slot(w, sg.item) * group + rank) * 2 + half;
+        return reinterpret_cast<float4*>(p.g.part) + (at * C::kRows + row) * 32;
+      };
+      int* arrived = p.g.arrived + ((sg.item - sched.first) * group + rank) * 8;
+      if (mine) {
+        float4* dst = part(sched.worker, m);
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          __stcg(dst + i, make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]));
+      }
+      __threadfence();
+      bool last;
+      if constexpr (SWIGLU) {
+        if (!pair_meet(&meet[q], met)) goto done;          // both halves are written
+        if (half == 0 && lane == 0) {
+          flag[(met & 1) * 4 + q] = atomicAdd(&arrived[q], 1) == c1 - c0;
+          __threadfence();
+        }
+        const int at = (met & 1) * 4 + q;
+        if (!pair_meet(&meet[q], met)) goto done;
+        last = flag[at] != 0;
+      } else {
+        int old = 0;
+        __syncwarp();
+        if (lane == 0) old = atomicAdd(&arrived[4 * half + q], 1);
+        last = __shfl_sync(0xffffffffu, old, 0) == c1 - c0;
+      }
+      if (!last) continue;
+      __threadfence();
+      // The last worker of the tile: lanes take columns now (4 each), rows one after another.
+      const int nr = min(32, it.cnt - 32 * q);
+      // 8 rows at a time, so that 8 loads (16 for two matrices) are under way at once.
+      for (int r0 = 0; r0 < nr; r0 += 8) {
+        float4 sum[8];                       // SwiGLU: gate columns in x, y and up columns in z, w
+#pragma unroll
+        for (int r = 0; r < 8; ++r) sum[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = c0; c <= c1; ++c) {
+          const float4* src = part(c, 32 * q + r0);
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            if (r0 + r >= nr) break;
+            float4 a;
+            if constexpr (SWIGLU) {
+              const float2* s2 = reinterpret_cast<const float2*>(src + 32 * r);
+              const float2 g = __ldcg(s2 + lane), u = __ldcg(s2 + 32 + lane);
+              a = make_float4(g.x, g.y, u.x, u.y);
+            } else {
+              a = __ldcg(src + 32 * r + lane);
+            }
+            sum[r].x += a.x;
+            sum[r].y += a.y;
+            sum[r].z += a.z;
+            sum[r].w += a.w;
+          }
+        }
+        if constexpr (SWIGLU) {
+          const int col0 = it.nt * 128 + 64 * half + 2 * lane;
+          float* mx = row_max + ((met & 1) * 4 + q) * 64;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            sum[r].x = col0 < rows ? swiglu_keep_nan(sum[r].x, sum[r].z, p.g.limit) : 0.f;
+            sum[r].y = col0 + 1 < rows ? swiglu_keep_nan(sum[r].y, sum[r].w, p.g.limit) : 0.f;
+            float top = max_nan(fabsf(sum[r].x), fabsf(sum[r].y));
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
+            if (lane == 0) mx[half * 32 + r] = top;
+          }
+          if (!pair_meet(&meet[q], met)) goto done;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            if (r0 + r >= nr) break;
+            float inv;
+            const float sc = fp8_group_scale(max_nan(mx[r], mx[32 + r]), &inv);
+            const size_t row = (size_t)it.row0 + 32 * q + r0 + r;
+            *reinterpret_cast<uint16_t*>(p.g.hq + row * ((size_t)p.RB * 128) + col0) = (uint16_t)__nv_cvt_float2_to_fp8x2(
+                make_float2(sum[r].x * inv, sum[r].y * inv), __NV_SATFINITE, __NV_E4M3);
+            if (half == 0 && lane == 0) p.g.hs[row * p.hs_ld + it.nt] = sc;
           }
         } else {
+          const int col0 = it.nt * 256 + 128 * half + 4 * lane;
+          const bool wide = rows % 4 == 0 && (reinterpret_cast<uintptr_t>(p.g.out) & 15) == 0;
 #pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (col0 + i < rows) dst[i] = out_of<OUT>(CBMOE_ACC(acc, i));
+          for (int r = 0; r < 8; ++r) {
+            if (r0 + r >= nr) break;
+            struct alignas(4 * sizeof(OUT)) Out4 {
+              OUT o[4];
+            } b = {{out_of<OUT>(sum[r].x), out_of<OUT>(sum[r].y), out_of<OUT>(sum[r].z), out_of<OUT>(sum[r].w)}};
+            OUT* dst = static_cast<OUT*>(p.g.out) + ((size_t)it.row0 + 32 * q + r0 + r) * rows + col0;
+            if (wide) {
+              if (col0 < rows) *reinterpret_cast<Out4*>(dst) = b;
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (col0 + i < rows) dst[i] = b.o[i];
+            }
+          }
         }
       }
-      ++local;
     }
   }
 done:
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
+  if constexpr (C::kPair) cluster_sync();    // neither CTA leaves while the other may reach into it
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    if constexpr (C::kPair) tmem_dealloc_pair(tmem, 512);
+    else tmem_dealloc(tmem, 512);
   }
 }
 
@@ -389,9 +641,11 @@ int launch_t(const Fp8Gemm& g, cudaStream_t stream) {
   p.g = g;
   p.KB = (g.K + kFp8Group - 1) / kFp8Group;
   p.RB = (g.rows + 127) / 128;
+  p.hs_ld = fp8_scale_stride(g.rows);
+  p.xs_wide = g.ldxs % 4 == 0 && (reinterpret_cast<uintptr_t>(g.xs) & 15) == 0;
   p.NT = SWIGLU ? p.RB : (p.RB + 1) / 2;
   CUtensorMap mx, m0, m1;
-  int rc = make_fp8_map(&mx, g.xq, g.K, g.x_rows, g.ldx, MT);
+  int rc = make_fp8_map(&mx, g.xq, g.K, g.x_rows, g.ldx, C::kRows);
   if (!rc) rc = make_fp8_map(&m0, g.w0, g.K, (long long)g.E * g.rows, g.ldw, 128);
   if (!rc) rc = make_fp8_map(&m1, SWIGLU ? g.w1 : g.w0, g.K, (long long)g.E * g.rows, g.ldw, 128);
   if (rc) return rc;
@@ -405,7 +659,20 @@ int launch_t(const Fp8Gemm& g, cudaStream_t stream) {
   }, &set);
   if (rc) return rc;
   prof_begin(kProfOther, stream);
-  CBMOE_CUDA_TRY(launch_pdl(kern, dim3(num_sms()), dim3(kFp8Threads), C::kSmem, stream, p, mx, m0, m1));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(C::kPair ? num_sms() & ~1 : num_sms());
+  cfg.blockDim = dim3(kFp8Threads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = C::kPair ? 2 : 1;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  CBMOE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, p, mx, m0, m1));
   prof_end(kProfOther, stream);
   CBMOE_CUDA_TRY(cudaGetLastError());
   return CBMOE_OK;
@@ -425,16 +692,30 @@ int blocks_of(int K) { return (K + kFp8Group - 1) / kFp8Group; }
 
 }  // namespace
 
-int fp8_pass_tokens(long long slots, int E) { return slots <= 32LL * E ? 32 : (slots <= 64LL * E ? 64 : 128); }
+int fp8_pass_tokens(long long slots, int E) {
+  return slots <= 32LL * E ? 32 : (slots <= 64LL * E ? 64 : (slots <= 128LL * E ? 128 : 256));
+}
+
+int fp8_device_errors(int clear, int* out_host) {
+  CBMOE_CUDA_TRY(cudaMemcpyFromSymbol(out_host, g_device_errors, sizeof(int)));
+  const int zero = 0;
+  if (clear && *out_host) CBMOE_CUDA_TRY(cudaMemcpyToSymbol(g_device_errors, &zero, sizeof(int)));
+  return CBMOE_OK;
+}
+
+size_t fp8_part_bytes(int mt) { return (size_t)num_sms() * 2 * (mt < 128 ? mt : 128) * kFp8TileN * 4; }
+
+int fp8_arrived() { return num_sms() * 8; }
 
 int launch_fp8_gemm(const Fp8Gemm& g, int mt, cudaStream_t s) {
   if (mt == 32) return launch_mt<32>(g, s);
   if (mt == 64) return launch_mt<64>(g, s);
-  return launch_mt<128>(g, s);
+  if (mt == 128) return launch_mt<128>(g, s);
+  return launch_mt<256>(g, s);
 }
 
-int launch_fp8_quantize(const void* x, int type, int N, int K, long long ldx, uint8_t* q, long long ldq, float* s,
-                        const int* row_slot, int k, int R, cudaStream_t stream) {
+int launch_fp8_quantize(const void* x, int type, int N, int K, long long ldx, uint8_t* q, long long ldq, float* s, int lds,
+                        const int* row_slot, int k, int R, int* zero, int n_zero, cudaStream_t stream) {
   const long long groups = (long long)N * blocks_of(K);
   long long blocks = (groups + 15) / 16, cap = (long long)num_sms() * 16;
   if (blocks > cap) blocks = cap;
@@ -443,13 +724,16 @@ int launch_fp8_quantize(const void* x, int type, int N, int K, long long ldx, ui
   prof_begin(kProfOther, stream);
   if (type == CBMOE_BF16)
     CBMOE_CUDA_TRY(launch_pdl(fp8_quantize_kernel<__nv_bfloat16>, dim3((int)blocks), dim3(256), 0, stream,
-                              static_cast<const __nv_bfloat16*>(x), N, K, ldx, vec, q, ldq, s, row_slot, k, R));
+                              static_cast<const __nv_bfloat16*>(x), N, K, ldx, vec, q, ldq, s, lds, row_slot, k, R, zero,
+                              n_zero));
   else if (type == CBMOE_F16)
     CBMOE_CUDA_TRY(launch_pdl(fp8_quantize_kernel<__half>, dim3((int)blocks), dim3(256), 0, stream,
-                              static_cast<const __half*>(x), N, K, ldx, vec, q, ldq, s, row_slot, k, R));
+                              static_cast<const __half*>(x), N, K, ldx, vec, q, ldq, s, lds, row_slot, k, R, zero,
+                              n_zero));
   else
     CBMOE_CUDA_TRY(launch_pdl(fp8_quantize_kernel<float>, dim3((int)blocks), dim3(256), 0, stream,
-                              static_cast<const float*>(x), N, K, ldx, vec, q, ldq, s, row_slot, k, R));
+                              static_cast<const float*>(x), N, K, ldx, vec, q, ldq, s, lds, row_slot, k, R, zero,
+                              n_zero));
   prof_end(kProfOther, stream);
   CBMOE_CUDA_TRY(cudaGetLastError());
   return CBMOE_OK;
@@ -457,19 +741,25 @@ int launch_fp8_quantize(const void* x, int type, int N, int K, long long ldx, ui
 
 namespace {
 
-// Workspace of a product with a quantised input: q [N][blocks * 128] | s [N][blocks].
+// Workspace of a product: partial sums | counters | q [N][blocks * 128] | s [N][blocks] (the last two where x is quantised
+// here).
 struct LinearWs {
-  size_t s, total;
+  size_t arrived, xq, xs, total;
+  int mt;
 };
-LinearWs linear_ws(int N, int K) {
+LinearWs linear_ws(int N, int K, bool ready) {
   LinearWs w;
-  w.s = lyr::align_up((size_t)N * blocks_of(K) * kFp8Group);
-  w.total = w.s + lyr::align_up((size_t)N * blocks_of(K) * 4);
+  w.mt = fp8_pass_tokens(N, 1);
+  w.arrived = lyr::align_up(fp8_part_bytes(w.mt));
+  w.xq = w.arrived + lyr::align_up((size_t)fp8_arrived() * 4);
+  w.xs = w.xq + (ready ? 0 : lyr::align_up((size_t)N * blocks_of(K) * kFp8Group));
+  w.total = w.xs + (ready ? 0 : lyr::align_up((size_t)N * fp8_scale_stride(K) * 4));
   return w;
 }
 
+// Workspace of the layer: plan | partial sums | counters (gate/up, down) | xq, xs (sorted rows) | hq, hs | slot outputs.
 struct ExpertsWs {
-  size_t plan, xq, xs, hq, hs, y, total;
+  size_t plan, part, arrived, xq, xs, hq, hs, y, total;
   int mt, Rp;
   lyr::PlanLayoutHost L;
 };
@@ -480,11 +770,13 @@ ExpertsWs experts_ws(int E, int H, int I, int N, int k, int y_type) {
   w.L = lyr::host_plan_layout(N, k, E, 1, w.mt);
   w.Rp = (int)S;                                        // blocks of one row: the sorted rows are [0, S)
   w.plan = 0;
-  w.xq = lyr::align_up((size_t)w.L.off[13] * 4);
+  w.part = lyr::align_up((size_t)w.L.off[13] * 4);
+  w.arrived = w.part + lyr::align_up(fp8_part_bytes(w.mt));
+  w.xq = w.arrived + lyr::align_up((size_t)fp8_arrived() * 2 * 4);
   w.xs = w.xq + lyr::align_up((size_t)S * blocks_of(H) * kFp8Group);
-  w.hq = w.xs + lyr::align_up((size_t)S * blocks_of(H) * 4);
+  w.hq = w.xs + lyr::align_up((size_t)S * fp8_scale_stride(H) * 4);
   w.hs = w.hq + lyr::align_up((size_t)S * blocks_of(I) * kFp8Group);
-  w.y = w.hs + lyr::align_up((size_t)S * blocks_of(I) * 4);
+  w.y = w.hs + lyr::align_up((size_t)S * fp8_scale_stride(I) * 4);
   w.total = w.y + lyr::align_up((size_t)S * H * (y_type == CBMOE_F32 ? 4 : 2));
   return w;
 }
@@ -511,13 +803,12 @@ extern "C" int cbmoe_fp8_quantize(const void* x, int type, int N, int K, long lo
   if (!type_ok(type) || N < 0 || K <= 0 || ldx < K || ldq < K) return CBMOE_ERR_INVALID;
   if (N == 0) return CBMOE_OK;
   if (!x || !q || !s) return CBMOE_ERR_INVALID;
-  return launch_fp8_quantize(x, type, N, K, ldx, q, ldq, s, nullptr, 1, N, stream);
+  return launch_fp8_quantize(x, type, N, K, ldx, q, ldq, s, blocks_of(K), nullptr, 1, N, nullptr, 0, stream);
 }
 
 extern "C" size_t cbmoe_fp8_linear_workspace_bytes(int N, int K, int rows, int x_type) {
   if (N < 0 || K <= 0 || rows <= 0) return 0;
-  if (x_type == CBMOE_E4M3) return 0;
-  return type_ok(x_type) ? linear_ws(N, K).total : 0;
+  return x_type == CBMOE_E4M3 || type_ok(x_type) ? linear_ws(N, K, x_type == CBMOE_E4M3).total : 0;
 }
 
 extern "C" int cbmoe_fp8_linear(const void* q, long long ldq, const float* s, int rows, int K, const void* x,
@@ -538,22 +829,28 @@ extern "C" int cbmoe_fp8_linear(const void* q, long long ldq, const float* s, in
   g.s0 = s;
   g.out = y;
   g.out_type = y_type;
+  const LinearWs W = linear_ws(N, K, ready);
+  if (!workspace || workspace_bytes < W.total || !aligned(workspace, 256)) return CBMOE_ERR_WORKSPACE;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  g.part = reinterpret_cast<float*>(ws);
+  g.arrived = reinterpret_cast<int*>(ws + W.arrived);
   if (ready) {
+    CBMOE_CUDA_TRY(cudaMemsetAsync(g.arrived, 0, (size_t)fp8_arrived() * 4, stream));
     g.xq = x;
     g.ldx = ldx;
     g.xs = xs;
+    g.ldxs = blocks_of(K);
   } else {
-    const LinearWs W = linear_ws(N, K);
-    if (!workspace || workspace_bytes < W.total || !aligned(workspace, 256)) return CBMOE_ERR_WORKSPACE;
-    uint8_t* xq = static_cast<uint8_t*>(workspace);
-    float* sc = reinterpret_cast<float*>(xq + W.s);
+    float* sc = reinterpret_cast<float*>(ws + W.xs);
+    g.ldxs = fp8_scale_stride(K);
     g.ldx = (long long)blocks_of(K) * kFp8Group;
-    const int rc = launch_fp8_quantize(x, x_type, N, K, ldx, xq, g.ldx, sc, nullptr, 1, N, stream);
+    const int rc = launch_fp8_quantize(x, x_type, N, K, ldx, ws + W.xq, g.ldx, sc, g.ldxs, nullptr, 1, N, g.arrived,
+                                       fp8_arrived(), stream);
     if (rc) return rc;
-    g.xq = xq;
+    g.xq = ws + W.xq;
     g.xs = sc;
   }
-  return launch_fp8_gemm(g, fp8_pass_tokens(N, 1), stream);
+  return launch_fp8_gemm(g, W.mt, stream);
 }
 
 extern "C" size_t cbmoe_fp8_experts_workspace_bytes(const cbmoe_fp8_experts* ex, int N, int k, int y_type) {
@@ -575,17 +872,21 @@ extern "C" int cbmoe_fp8_experts_apply(const cbmoe_fp8_experts* ex, const uint16
   int rc = launch_route_plan(idx, w, N, k, ex->E, 1, W.mt, plan, stream, nullptr, 0);
   if (rc) return rc;
   const int32_t* row_slot = plan + W.L.off[9];
+  int* arrived = reinterpret_cast<int*>(ws + W.arrived);
   Fp8Gemm g{};
   g.E = ex->E;
   g.rows = ex->I;
   g.K = ex->H;
   g.ldx = (long long)blocks_of(ex->H) * kFp8Group;
   g.x_rows = W.Rp;
+  g.ldxs = fp8_scale_stride(ex->H);
   g.xq = ws + W.xq;
   g.xs = reinterpret_cast<const float*>(ws + W.xs);
-  rc = launch_fp8_quantize(x, CBMOE_BF16, N, ex->H, ex->H, ws + W.xq, g.ldx, reinterpret_cast<float*>(ws + W.xs),
-                           row_slot, k, W.Rp, stream);
+  rc = launch_fp8_quantize(x, CBMOE_BF16, N, ex->H, ex->H, ws + W.xq, g.ldx, reinterpret_cast<float*>(ws + W.xs), g.ldxs,
+                           row_slot, k, W.Rp, arrived, 2 * fp8_arrived(), stream);
   if (rc) return rc;
+  g.part = reinterpret_cast<float*>(ws + W.part);
+  g.arrived = arrived;
   g.w0 = ex->gate;
   g.w1 = ex->up;
   g.ldw = ex->ld_in;
@@ -606,11 +907,13 @@ extern "C" int cbmoe_fp8_experts_apply(const cbmoe_fp8_experts* ex, const uint16
   d.xq = g.hq;
   d.ldx = (long long)blocks_of(ex->I) * kFp8Group;
   d.xs = g.hs;
+  d.ldxs = fp8_scale_stride(ex->I);
   d.w0 = ex->down;
   d.w1 = nullptr;
   d.ldw = ex->ld_down;
   d.s0 = ex->down_s;
   d.s1 = nullptr;
+  d.arrived = arrived + fp8_arrived();
   d.hq = nullptr;
   d.hs = nullptr;
   d.out = ws + W.y;

@@ -45,7 +45,8 @@ struct Fp8Gemm {
   const void* xq;          // e4m3 [x_rows][ldx]
   long long ldx;
   int x_rows;
-  const float* xs;         // [x_rows][ceil(K / 128)]
+  const float* xs;         // [x_rows][ldxs], ldxs >= ceil(K / 128)
+  int ldxs;
   const void* w0;          // e4m3 [E][rows][ldw]; w1: up, beside w0 = gate (SwiGLU), else null
   const void* w1;
   long long ldw;
@@ -58,16 +59,25 @@ struct Fp8Gemm {
   float limit;             // SwiGLU clamp
   void* out;               // one matrix: [x_rows][rows] of out_type
   int out_type;
-  uint8_t* hq;             // SwiGLU: e4m3 [x_rows][ceil(rows / 128) * 128] and its scales [x_rows][ceil(rows / 128)]
+  float* part;             // fp8_part_bytes(mt): partial sums of tiles that several CTAs share
+  int* arrived;            // fp8_arrived() counters, zero before the launch
+  uint8_t* hq;             // SwiGLU: e4m3 [x_rows][ceil(rows / 128) * 128] and its scales [x_rows][fp8_scale_stride(rows)]
   float* hs;
 };
 
-// Token rows per pass of the product kernel: 32, 64 or 128.
+// Row stride of the scales that the library keeps for itself: four blocks are one 16-byte load.
+inline int fp8_scale_stride(int K) { return ((K + kFp8Group - 1) / kFp8Group + 3) & ~3; }
+// This file's own error word (common.cuh), after the device is synchronized.
+int fp8_device_errors(int clear, int* out_host);
+// Token rows per pass of the product kernel: 32, 64, 128 or 256 (a pair of CTAs).
 int fp8_pass_tokens(long long slots, int E);
+size_t fp8_part_bytes(int mt);
+int fp8_arrived();         // counters of one launch: 8 for each tile that can be shared (fewer than the SMs)
 int launch_fp8_gemm(const Fp8Gemm& g, int mt, cudaStream_t s);
 // x [N][K] (row stride ldx elements) -> e4m3 rows q (stride ldq bytes, columns K.. up to ldq zero where a unit of 8
-// reaches past K) and scales s [..][ceil(K / 128)]; with row_slot, row n goes to the k rows row_slot[n][:] in [0, R).
-int launch_fp8_quantize(const void* x, int type, int N, int K, long long ldx, uint8_t* q, long long ldq, float* s,
-                        const int* row_slot, int k, int R, cudaStream_t stream);
+// reaches past K) and scales s [..][lds]; with row_slot, row n goes to the k rows row_slot[n][:] in [0, R).
+// Clears zero[0, n_zero) on the way (the counters of the products that follow).
+int launch_fp8_quantize(const void* x, int type, int N, int K, long long ldx, uint8_t* q, long long ldq, float* s, int lds,
+                        const int* row_slot, int k, int R, int* zero, int n_zero, cudaStream_t stream);
 
 }  // namespace cbmoe
