@@ -44,6 +44,16 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
+// Arrive where `yes` is set, as a predicated instruction: no branch that the warp has to come back from.
+__device__ __forceinline__ void mbar_arrive_if(uint64_t* bar, bool yes) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %1, 0;\n\t"
+      "@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}\n" ::"r"(smem_addr(bar)),
+      "r"((int)yes)
+      : "memory");
+}
+
 __device__ __forceinline__ void mbar_arrive_expect_tx(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes)
                : "memory");
@@ -77,14 +87,26 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
   return true;
 }
 
+// The same wait in a few instructions, for loops that have to stay in the instruction cache: a try that fails has
+// suspended the thread for about 4 us (measured), so 2^20 of them are the limit of kWaitLimitNs. The caller records a
+// wait that gave up (CBMOE_DEVERR_TIMEOUT) on its way out.
+__device__ __forceinline__ bool mbar_wait_brief(uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
+  for (int i = 0; i < (1 << 20); ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return false;
+}
+
 // Arrive on the barrier at the same shared-memory offset of CTA `rank` of the cluster. Orders no ordinary memory accesses
 // between the CTAs: it tells of finished TMA loads and TMEM reads only.
-__device__ __forceinline__ void mbar_arrive_remote(uint64_t* bar, uint32_t rank) {
+__device__ __forceinline__ void mbar_arrive_remote(uint64_t* bar, uint32_t rank, bool yes = true) {
   asm volatile(
       "{\n\t.reg .b32 a;\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %2, 0;\n\t"
       "mapa.shared::cluster.u32 a, %0, %1;\n\t"
-      "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}\n" ::"r"(smem_addr(bar)),
-      "r"(rank)
+      "@p mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}\n" ::"r"(smem_addr(bar)),
+      "r"(rank), "r"((int)yes)
       : "memory");
 }
 

@@ -5,24 +5,24 @@
 // fp8_gemm_kernel, one CTA per SM, 12 warps:
 //   warp 0      TMA producer: per 128-column block the tile's MT x 128 B of tokens and 2 x 128 x 128 B of weights (128-byte
 //               swizzle), into a ring of stages
-//   warp 1      TMEM owner and MMA issuer (one thread): 4 tcgen05.mma kind::f8f6f4 (M 128 x N 256 x K 32) per block into
-//               one of two 256-column accumulators
+//   warp 1      TMEM owner and MMA issuer (one elected lane): 4 tcgen05.mma kind::f8f6f4 (M 128 x N 256 x K 32) per block
+//               into one of two 256-column accumulators (tiles of 128 or 64 weight rows: 2 or 4 blocks side by side)
 //   warps 4-11  promotion and epilogue: a block's 128 x 256 partial sums leave TMEM while the tensor core works on the next
 //               block; acc += partial * (sx * sw) in fp32 registers (32 rows x 128 columns per warp). Tokens are the M side,
 //               so a thread owns one token row: both scales are scalars for its columns. These warps take the registers
-//               that the first warpgroup gives up (128 accumulators + two 32-column loads in turn a thread).
+//               that the first warpgroup gives up (128 accumulators and a 16-column load a thread).
 // The block's partial sum is exact enough to be added as it is: e4m3 products are exact in fp32 and the tensor core sums
 // them in fp32 (measured: 1e-8 relative over K = 128).
 // With many rows (MT = 256) two CTAs of a cluster work as a pair (cta_group::2, M = 256): each brings 128 tokens and half
-// of the weight tile, so a block costs an SM 32 KB of shared-memory writes and 32 KB of operand reads where a CTA alone
-// costs it 48 and 48, which at 128 B a clock is more than the 512 clocks of its MMAs (measured at 4096 x 5120 x 12288:
-// alone 1300 clocks a block, 1070 with the promotion left out).
+// of the weight tile, 32 KB of loads a block where a CTA alone takes 48. What bounds it (one B200, 4096 x 12288 -> 9472):
+// 1.88-1.92 PFLOP/s; a loop of its own that only loads and multiplies takes 380 us of the 500 because the clock falls to
+// 1.06 GHz under the power cap, reading TMEM adds 45 us, the fp32 multiply-adds 45 us; the rest are the tiles' ends.
 // With two matrices (gate, up: 128 columns each) the epilogue forms swiglu_clamped(gate, up), takes each row's maximum
 // over its 128 columns and stores e4m3 codes and the scale: the down product's input, never in 16 bits.
-// Work: whole waves of output tiles, one tile per CTA; the tiles left over are cut along K into equal ranges of blocks, one
-// per CTA (Fp8Sched), so that few rows (a single token: all of the time) still use every SM and the memory behind it. A
-// tile's ranges leave fp32 partial sums in the workspace; the last to arrive adds them in range order (the same bits on
-// every call) and runs the epilogue.
+// Work: whole waves of output tiles, one tile per CTA (pair). Tiles left over are cut along K into equal ranges of blocks
+// where that pays (Fp8Sched): always for pairs, which wait for arithmetic; else only where there are fewer tiles than half
+// of the SMs. A tile's ranges leave fp32 partial sums in the workspace; the last to arrive adds them in range order (the
+// same bits on every call) and runs the epilogue. Few tokens take narrower tiles, so that enough SMs stream weights.
 // Every wait is bounded; a role that gives up sets CBMOE_DEVERR_TIMEOUT and falls through to the final barrier.
 #define CBMOE_OWN_UNIT
 #include <cudaTypedefs.h>
@@ -106,31 +106,52 @@ __global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__
   }
 }
 
+// Scales that come with codes [N][KB] -> rows padded to whole 16-byte groups; clears the product's counters on the way.
+__global__ void __launch_bounds__(256) fp8_scales_kernel(const float* __restrict__ xs, int N, int KB, int ld,
+                                                         float* __restrict__ out, int* __restrict__ zero, int n_zero) {
+  griddep_wait();
+  griddep_launch();
+  const long long total = (long long)N * ld, at = blockIdx.x * 256LL + threadIdx.x, step = gridDim.x * 256LL;
+  for (long long i = at; i < n_zero; i += step) zero[i] = 0;
+  for (long long i = at; i < total; i += step) {
+    const long long n = i / ld;
+    const int kb = (int)(i - n * ld);
+    out[i] = kb < KB ? xs[n * KB + kb] : 0.f;
+  }
+}
+
 // --------------------------------------------------------------------------------------------------- product
 constexpr int kFp8Threads = 12 * 32;
 constexpr int kW0 = 4;                                   // first promotion warp
-constexpr int kBHalf = 128 * 128;                        // 128 weight rows of one block
 constexpr int kRegsIdle = 40, kRegsWork = 232;           // 128 * 40 + 256 * 232 = 384 * 168, the launch's registers
 
-template <int MT>
+// MT tokens and TN weight rows per tile (two matrices: TN / 2 of each).
+template <int MT, int TN>
 struct Fp8Cfg {
   static constexpr bool kPair = MT == 256;               // two CTAs, 128 tokens each
   static constexpr int kRows = kPair ? 128 : MT;         // tokens of a CTA's tile
   static constexpr int kATile = kRows * 128;
-  static constexpr int kStage = kATile + (kPair ? 1 : 2) * kBHalf;
-  static constexpr int kNStage = kPair ? 6 : (MT == 128 ? 4 : (MT == 64 ? 5 : 6));
-  static constexpr int kBarOff = kNStage * kStage;
-  static constexpr int kMaxOff = kBarOff + 256;          // row maxima [2][4 quadrants][2 halves][32] f32
+  static constexpr int kBTile = (kPair ? TN / 2 : TN) * 128;
+  // Column blocks per stage and per accumulator (256 columns in all): a hand-over costs some 500 clocks of the issuer and
+  // of the promotion warps whatever its size, so narrow tiles take several blocks at once.
+  static constexpr int kU = 256 / TN;
+  static constexpr int kStage = kU * (kATile + kBTile);
+  static constexpr int kRest = 1024 + 2048 + 32 + 512;
+  static constexpr int kNStage = (227 * 1024 - kRest) / kStage < 16 ? (227 * 1024 - kRest) / kStage : 16;
+  static constexpr int kMaxOff = kNStage * kStage;       // row maxima [2][4 quadrants][2 halves][32] f32
   static constexpr int kFlagOff = kMaxOff + 2048;        // [2][4] int
-  static constexpr int kSmem = 1024 + kFlagOff + 32;
+  static constexpr int kBarOff = kFlagOff + 32;
+  static constexpr int kSmem = 1024 + kBarOff + 512;
+  static_assert((2 * kNStage + 9) * 8 <= 512, "barriers");
   static_assert(kSmem <= 227 * 1024, "shared memory budget");
+  // The tensor core reads 128 rows of the M side whatever MT: past a block's tokens that is still its stage.
+  static_assert((kU - 1) * kATile + 128 * 128 <= kStage, "M side inside the stage");
 };
 
 struct Fp8Params {
   Fp8Gemm g;
   int KB, RB, NT;          // column blocks, 128-row blocks per matrix, output tiles per pass
   int hs_ld;               // row stride of hs
-  int xs_wide;             // xs rows are 16-byte aligned
 };
 
 struct Fp8Item {
@@ -149,20 +170,22 @@ __device__ __forceinline__ Fp8Item fp8_item(const Fp8Params& p, int item) {
   return {p.g.pass_expert[pass], p.g.pass_row0[pass], p.g.pass_cnt[pass], nt};
 }
 
-// A worker's (a CTA's, or a pair's) share of the tiles, in segments (tile, blocks [kb0, kb1)).
+// A worker's (a CTA's, or a pair's) share of the tiles, in segments (tile, units [kb0, kb1) of kU column blocks).
 struct Fp8Seg {
   int item, kb0, kb1;
 };
 struct Fp8Sched {
   int waves, first, KB, chunk, u, u1, i, worker, G;
 
-  // Ranges shorter than 4 blocks would spend more on joining them than on their sums.
-  // Worker `w` of `G` (a CTA, or a pair).
-  __device__ __forceinline__ Fp8Sched(int n_items, int kb, int w, int g) : KB(kb), i(0), worker(w), G(g) {
+  // Worker `w` of `g` (a CTA, or a pair). Pairs cut whatever is left over: with many rows the SMs' arithmetic is what
+  // counts. Alone, a CTA with few rows waits for memory, which half of the SMs keep busy: tiles are cut only where there
+  // are fewer than that. Ranges below 4 (8) blocks would spend more on joining than on their sums.
+  __device__ __forceinline__ Fp8Sched(int n_items, int kb, int w, int g, bool pair) : KB(kb), i(0), worker(w), G(g) {
     const int rem = n_items % G;
     waves = n_items / G;
     first = waves * G;
-    chunk = max((rem * KB + G - 1) / G, min(KB, 4));
+    chunk = pair ? 4 : (waves == 0 && 2 * rem <= G ? 8 : KB);
+    chunk = max((rem * KB + G - 1) / G, min(KB, chunk));
     u = min(rem * KB, worker * chunk);
     u1 = min(rem * KB, u + chunk);
   }
@@ -202,6 +225,33 @@ __device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
                : "memory");
 }
 
+// A thread's W sums to the columns [col0, col0 + W) of its row, as far as the matrix goes: whole 32-byte sectors where
+// rows allow them (a lane per row, so narrower stores would leave the sectors in pieces).
+template <int W, typename OUT, int N>
+__device__ __forceinline__ void store_row(void* out, size_t row, int rows, int col0, const float (&acc)[N]) {
+  const int end = min(rows - col0, W);
+  OUT* dst = static_cast<OUT*>(out) + row * rows + col0;
+  constexpr int kU = 32 / (int)sizeof(OUT);
+  if (rows % kU == 0 && (reinterpret_cast<uintptr_t>(out) & 31) == 0) {
+#pragma unroll
+    for (int u = 0; u < W / kU; ++u) {
+      if (u * kU < end) {
+        union {
+          uint32_t w[8];
+          OUT o[kU];
+        } b;
+#pragma unroll
+        for (int i = 0; i < kU; ++i) b.o[i] = out_of<OUT>(acc[u * kU + i]);
+        store32(dst + u * kU, b.w);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+      if (i < end) dst[i] = out_of<OUT>(acc[i]);
+  }
+}
+
 // silu(min(g, L)) * clip(u, -L, L) (model.py:119-122) that keeps a NaN, so that a bad row shows.
 __device__ __forceinline__ float swiglu_keep_nan(float g, float u, float limit) {
   g = g > limit ? limit : g;
@@ -213,33 +263,31 @@ __device__ __forceinline__ float swiglu_keep_nan(float g, float u, float limit) 
 __device__ __forceinline__ bool pair_meet(uint64_t* bar, uint32_t& n) {
   __syncwarp();
   if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
-  return mbar_wait(bar, n++ & 1);
+  return mbar_wait_brief(bar, n++ & 1);
 }
 
-template <int MT, bool SWIGLU, typename OUT>
+template <int MT, int TN, bool SWIGLU>
 __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const Fp8Params p,
                                                                   const __grid_constant__ CUtensorMap map_x,
                                                                   const __grid_constant__ CUtensorMap map_w0,
                                                                   const __grid_constant__ CUtensorMap map_w1) {
-  using C = Fp8Cfg<MT>;
+  using C = Fp8Cfg<MT, TN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOff);
-  uint64_t* empty = full + C::kNStage;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBarOff);   // [kNStage]
+  uint64_t* empty = full + C::kNStage;      // [kNStage]
   uint64_t* d_full = empty + C::kNStage;    // [2]
   uint64_t* d_empty = d_full + 2;           // [2]
   uint64_t* meet = d_empty + 2;             // [4]
-  uint64_t* peer = meet + 4;                // [kNStage] pair, in rank 0: the other CTA's stage is full
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(peer + C::kNStage);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(meet + 4);
   float* row_max = reinterpret_cast<float*>(smem + C::kMaxOff);
   volatile int* flag = reinterpret_cast<volatile int*>(smem + C::kFlagOff);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kNStage; ++i) {
-      mbar_init(&full[i], 1);
+      mbar_init(&full[i], C::kPair && cluster_rank() == 0 ? 2 : 1);   // rank 0 of a pair: the other CTA's loads too
       mbar_init(&empty[i], 1);
-      mbar_init(&peer[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&d_full[i], 1);
@@ -265,30 +313,47 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const Fp8Param
   const int rank = C::kPair ? (int)cluster_rank() : 0, group = C::kPair ? 2 : 1;
   griddep_wait();
   griddep_launch();
+  const int KBU = (p.KB + C::kU - 1) / C::kU;               // units of a whole sum
+  auto schedule = [&]() { return Fp8Sched(fp8_items<MT>(p), KBU, blockIdx.x / group, gridDim.x / group, C::kPair); };
 
   if (warp < kW0) {
     regs_give_up<kRegsIdle>();
-    Fp8Sched sched(fp8_items<MT>(p), p.KB, blockIdx.x / group, gridDim.x / group);
-    Fp8Seg sg;
     // Whole warps walk these loops and one elected lane issues: addresses and descriptors stay in uniform registers, which
     // halves the instructions of an issue (measured beside the promotion warps: 870 -> 760 clocks a block).
     int st = 0;
     uint32_t ph = 0;
     if (warp == 0) {
-      while (sched.next(sg)) {
-        const Fp8Item it = fp8_item<MT>(p, sg.item);
-        const int wrow = it.e * p.g.rows + it.nt * (SWIGLU ? 128 : 256), xrow = it.row0 + 128 * rank;
+      auto weights = [&](const Fp8Item& it, int u, int st) {
+        const int wrow = it.e * p.g.rows + it.nt * (SWIGLU ? TN / 2 : TN);
+        uint8_t* b = smem + st * C::kStage + C::kU * C::kATile;
+#pragma unroll
+        for (int j = 0; j < C::kU; ++j) {
+          const int x = (u * C::kU + j) * kFp8Group;        // past K: zeros
+          if (!C::kPair || rank == 0) tma_load_2d(b + j * C::kBTile, &map_w0, x, wrow, &full[st]);
+          if (!C::kPair || rank == 1)
+            tma_load_2d(b + j * C::kBTile + (C::kPair ? 0 : TN / 2 * 128), SWIGLU ? &map_w1 : &map_w0, x,
+                        SWIGLU ? wrow : wrow + TN / 2, &full[st]);
+        }
+      };
+      Fp8Sched sched = schedule();
+      Fp8Seg sg, sn;
+      bool have = sched.next(sg);
+      Fp8Item it{};
+      if (have) it = fp8_item<MT>(p, sg.item);
+      while (have) {
+        const bool have_n = sched.next(sn);
+        Fp8Item itn{};
+        if (have_n) itn = fp8_item<MT>(p, sn.item);         // under way while this segment's loads are issued
+        const int xrow = it.row0 + 128 * rank;
 #pragma unroll 1
-        for (int kb = sg.kb0; kb < sg.kb1; ++kb) {
-          if (!mbar_wait(&empty[st], ph ^ 1)) goto done;
-          uint8_t* a = smem + st * C::kStage;
+        for (int u = sg.kb0; u < sg.kb1; ++u) {
+          if (!mbar_wait_brief(&empty[st], ph ^ 1)) goto late;
           if (elect_one()) {
             mbar_arrive_expect_tx(&full[st], C::kStage);
-            tma_load_2d(a, &map_x, kb * kFp8Group, xrow, &full[st]);
-            if (!C::kPair || rank == 0) tma_load_2d(a + C::kATile, &map_w0, kb * kFp8Group, wrow, &full[st]);
-            if (!C::kPair || rank == 1)
-              tma_load_2d(a + C::kATile + (C::kPair ? 0 : kBHalf), SWIGLU ? &map_w1 : &map_w0, kb * kFp8Group,
-                          SWIGLU ? wrow : wrow + 128, &full[st]);
+            weights(it, u, st);
+#pragma unroll
+            for (int j = 0; j < C::kU; ++j)
+              tma_load_2d(smem + st * C::kStage + j * C::kATile, &map_x, (u * C::kU + j) * kFp8Group, xrow, &full[st]);
           }
           __syncwarp();
           if (++st == C::kNStage) {
@@ -296,14 +361,19 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const Fp8Param
             ph ^= 1;
           }
         }
+        sg = sn;
+        it = itn;
+        have = have_n;
       }
     } else if (warp == 1 && rank == 1) {
       // The pair's MMAs are issued by rank 0: tell it which of this CTA's stages are full.
+      Fp8Sched sched = schedule();
+      Fp8Seg sg;
       while (sched.next(sg)) {
 #pragma unroll 1
         for (int kb = sg.kb0; kb < sg.kb1; ++kb) {
-          if (!mbar_wait(&full[st], ph)) goto done;
-          if (elect_one()) mbar_arrive_remote(&peer[st], 0);
+          if (!mbar_wait_brief(&full[st], ph)) goto late;
+          if (elect_one()) mbar_arrive_remote(&full[st], 0);
           __syncwarp();
           if (++st == C::kNStage) {
             st = 0;
@@ -312,23 +382,26 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const Fp8Param
         }
       }
     } else if (warp == 1) {
-      constexpr uint32_t idesc = idesc_e4m3(C::kPair ? 256 : 128, kFp8TileN);
+      Fp8Sched sched = schedule();
+      Fp8Seg sg;
+      constexpr uint32_t idesc = idesc_e4m3(C::kPair ? 256 : 128, TN);
       const uint64_t desc0 = sw128_desc(smem_addr(smem));
       uint32_t buf = 0, dph = 1;
       while (sched.next(sg)) {
 #pragma unroll 1
-        for (int kb = sg.kb0; kb < sg.kb1; ++kb) {
-          if (!mbar_wait(&d_empty[buf], dph) || !mbar_wait(&full[st], ph)) goto done;
-          if (C::kPair && !mbar_wait(&peer[st], ph)) goto done;
+        for (int u = sg.kb0; u < sg.kb1; ++u) {
+          if (!mbar_wait_brief(&d_empty[buf], dph) || !mbar_wait_brief(&full[st], ph)) goto late;
           tc_fence_after();
-          // Rows kRows.. of the M side are whatever follows in the stage (weights): their sums are never read.
-          const uint64_t ad = desc0 + (uint32_t)st * (C::kStage >> 4), bd = ad + (C::kATile >> 4);
-          const uint32_t d = tmem + buf * kFp8TileN;
+          // Rows kRows.. of the M side are whatever follows in the stage: their sums are never read.
+          const uint64_t a0 = desc0 + (uint32_t)(st * (C::kStage >> 4)), b0 = a0 + (C::kU * C::kATile >> 4);
+          const uint32_t d = tmem + buf * 256;
           if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
-              if constexpr (C::kPair) umma_fp8_pair(d, ad + 2 * kk, bd + 2 * kk, idesc, kk != 0);
-              else umma_fp8(d, ad + 2 * kk, bd + 2 * kk, idesc, kk != 0);
+            for (int kk = 0; kk < 4 * C::kU; ++kk) {
+              const uint64_t ad = a0 + (kk / 4) * (C::kATile >> 4) + 2 * (kk % 4);
+              const uint64_t bd = b0 + (kk / 4) * (C::kBTile >> 4) + 2 * (kk % 4);
+              if constexpr (C::kPair) umma_fp8_pair(d, ad, bd, idesc, kk % 4 != 0);
+              else umma_fp8(d + (kk / 4) * TN, ad, bd, idesc, kk % 4 != 0);
             }
             if constexpr (C::kPair) {
               umma_commit_pair(&empty[st]);
@@ -350,119 +423,164 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const Fp8Param
     }
   } else {
     regs_take<kRegsWork>();
-    Fp8Sched sched(fp8_items<MT>(p), p.KB, blockIdx.x / group, gridDim.x / group);
-    Fp8Seg sg;
+    Fp8Sched sched = schedule();
     const int q = warp & 3;                  // TMEM lane quadrant this warp may read
     const int half = (warp - kW0) >> 2;
+    const int m = 32 * q + lane;             // this thread's row of the CTA's tile
     uint32_t n = 0, met = 0;
     auto d_read = [&](int buf) {             // to the CTA that issues the MMAs
-      if (rank == 0) mbar_arrive(&d_empty[buf]);
-      else mbar_arrive_remote(&d_empty[buf], 0);
+      __syncwarp();
+      if constexpr (C::kPair) mbar_arrive_remote(&d_empty[buf], 0, lane == 0);
+      else mbar_arrive_if(&d_empty[buf], lane == 0);
     };
-    while (sched.next(sg)) {
-      Fp8Item it = fp8_item<MT>(p, sg.item);
+    auto item_of = [&](const Fp8Seg& s) {
+      Fp8Item it = fp8_item<MT>(p, s.item);
       it.row0 += 128 * rank;                 // this CTA's rows of the tile
       it.cnt -= 128 * rank;
-      const int m = 32 * q + lane;
+      return it;
+    };
+    // A tile's place in the plan is fetched while the tile before it is summed.
+    Fp8Seg sg{}, sn{};
+    Fp8Item it{}, itn{};
+    bool have = sched.next(sg);
+    if (have) it = item_of(sg);
+    while (have) {
       const bool live = 32 * q < it.cnt, mine = m < it.cnt;
       const size_t xrow = mine ? (size_t)it.row0 + m : 0;
-      const float* sx = p.g.xs + xrow * p.g.ldxs;
-      const float *sa, *sb;                  // scales of this thread's columns 0-63 and 64-127
-      if constexpr (SWIGLU) {
-        sa = p.g.s0 + ((size_t)it.e * p.RB + it.nt) * p.KB;
-        sb = p.g.s1 + ((size_t)it.e * p.RB + it.nt) * p.KB;
-      } else {
-        sa = p.g.s0 + ((size_t)it.e * p.RB + min(2 * it.nt + half, p.RB - 1)) * p.KB;
-        sb = sa;
-      }
-      float acc[128];
+      const bool have_n = sched.next(sn);
+      if (have_n) itn = item_of(sn);         // under way while this tile is summed
+      float acc[TN / 2];
 #pragma unroll
-      for (int i = 0; i < 128; ++i) acc[i] = 0.f;
-      // Scales come four blocks ahead of their use (a load's latency under the tiles' traffic is longer than a block):
-      // this row's own, four blocks at a time; the weights', one block per lane.
-      auto row_scales = [&](int kb) {
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (p.xs_wide && kb % 4 == 0) {
-          if (kb < sg.kb1) v = *reinterpret_cast<const float4*>(sx + kb);
-        } else {
-          if (kb < sg.kb1) v.x = sx[kb];
-          if (kb + 1 < sg.kb1) v.y = sx[kb + 1];
-          if (kb + 2 < sg.kb1) v.z = sx[kb + 2];
-          if (kb + 3 < sg.kb1) v.w = sx[kb + 3];
-        }
-        return v;
-      };
-      float4 xn = row_scales(sg.kb0), xc = xn;
-      float wa = 0.f, wb = 0.f, wa_n = 0.f, wb_n = 0.f;
-      if (sg.kb0 + lane < sg.kb1) {
-        wa_n = sa[sg.kb0 + lane];
-        if constexpr (SWIGLU) wb_n = sb[sg.kb0 + lane];
-      }
+      for (int i = 0; i < TN / 2; ++i) acc[i] = 0.f;
+      // This row's scales, four blocks at a time (rows are padded to whole groups: fp8_scale_stride), and the weights', a
+      // block per lane: of this half's 128-row block, or of gate and up. Fetched at least four blocks ahead of their use: a
+      // load's latency under the tiles' traffic is longer than a block.
+      const float* sx = p.g.xs + xrow * p.g.ldxs;
+      const int blk = SWIGLU ? it.nt : min((it.nt * TN + half * (TN / 2)) / 128, p.RB - 1), kb0 = sg.kb0 * C::kU;
+      const float* sa = p.g.s0 + ((size_t)it.e * p.RB + blk) * p.KB;
+      const float* sb = SWIGLU ? p.g.s1 + ((size_t)it.e * p.RB + blk) * p.KB : sa;
+      auto row_scales = [&](int kb) { return *reinterpret_cast<const float4*>(sx + min(kb, (p.KB - 1) & ~3)); };
+      float4 xn = row_scales(kb0 & ~3), xc = xn;
+      float wa = 0.f, wb = 0.f;
+      float wa_n = kb0 + lane < p.KB ? sa[kb0 + lane] : 0.f, wb_n = SWIGLU && kb0 + lane < p.KB ? sb[kb0 + lane] : 0.f;
       // Not unrolled: 128 multiply-adds a turn fill the instruction cache that the MMA issuer shares.
 #pragma unroll 1
-      for (int kb = sg.kb0; kb < sg.kb1; ++kb) {
-        const int at = kb - sg.kb0;
-        if (at % 4 == 0) {
+      for (int u = sg.kb0; u < sg.kb1; ++u, ++n) {
+        const int kb = u * C::kU, i32 = (kb - kb0) % 32, buf = n & 1;
+        if (kb % 4 == 0 || kb == kb0) {
           xc = xn;
-          xn = row_scales(kb + 4);
+          xn = row_scales((kb & ~3) + 4);
+          if (kb % 4 >= 2) xc.x = xc.z, xc.y = xc.w;         // a range that begins inside a group
+          if (kb % 2 != 0) xc.x = xc.y, xc.y = xc.z, xc.z = xc.w;
         }
-        if (at % 32 == 0) {
+        if (i32 == 0) {
           wa = wa_n, wb = wb_n;
-          if (kb + 32 + lane < sg.kb1) {
-            wa_n = sa[kb + 32 + lane];
-            if constexpr (SWIGLU) wb_n = sb[kb + 32 + lane];
+          const int k = kb + 32 + lane;
+          if (k < p.KB) {
+            wa_n = sa[k];
+            if constexpr (SWIGLU) wb_n = sb[k];
           }
         }
-        const int buf = n & 1;
-        const float fa = xc.x * __shfl_sync(0xffffffffu, wa, at);
-        const float fb = SWIGLU ? xc.x * __shfl_sync(0xffffffffu, wb, at) : fa;
-        xc.x = xc.y, xc.y = xc.z, xc.z = xc.w;
-        if (!mbar_wait(&d_full[buf], (n >> 1) & 1)) goto done;
-        ++n;
+        float fa[C::kU], fb = 0.f;
+#pragma unroll
+        for (int j = 0; j < C::kU; ++j) {
+          fa[j] = (j == 0 ? xc.x : (j == 1 ? xc.y : (j == 2 ? xc.z : xc.w))) * __shfl_sync(0xffffffffu, wa, i32 + j);
+          if (C::kU > 1 && kb + j >= p.KB) fa[j] = 0.f;      // past K the products are zero, the scales are not
+        }
+        if constexpr (SWIGLU) fb = xc.x * __shfl_sync(0xffffffffu, wb, i32);
+        if constexpr (C::kU == 1) xc.x = xc.y, xc.y = xc.z, xc.z = xc.w;
+        if constexpr (C::kU == 2) xc.x = xc.z, xc.y = xc.w;
+        if (!mbar_wait_brief(&d_full[buf], (n >> 1) & 1)) goto late;
         tc_fence_after();
         if (live) {
-          const uint32_t t0 = tmem + buf * kFp8TileN + ((uint32_t)(32 * q) << 16);
+          const uint32_t t0 = tmem + buf * 256 + ((uint32_t)(32 * q) << 16);
           // 16 columns at a time: the two warps of a scheduler take turns between a load and its multiply-adds, and
-          // 128 + 16 registers a thread leave nothing to spill (loads of 32 columns or two in flight measured the same
-          // in a loop of their own, 350-370 clocks a block, and spilled here).
+          // 128 + 16 registers a thread leave nothing to spill (one spilled register in this loop costs more than any
+          // longer load gains).
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {       // 0-3 gate and 4-7 up; or 8 in a row
+          for (int c = 0; c < 8; ++c) {         // SwiGLU: 0-3 gate, 4-7 up; else kU blocks of TN / 32
             float v[16];
-            tmem_ld16(t0 + (SWIGLU ? (c < 4 ? 64 * half + 16 * c : 64 + 64 * half + 16 * c) : 128 * half + 16 * c), v);
-            if (c == 7) {                     // all of this block is in registers
+            const int j = SWIGLU ? 0 : 16 * c / (TN / 2), at = SWIGLU ? 16 * c : 16 * c % (TN / 2);
+            tmem_ld16(t0 + (SWIGLU ? (c < 4 ? 0 : 64) + 64 * half + 16 * c : j * TN + TN / 2 * half + at), v);
+            if (c == 7) {                       // all of this unit is in registers
               tc_fence_before();
-              __syncwarp();
-              if (lane == 0) d_read(buf);
+              d_read(buf);
             }
+            const float f = SWIGLU && c >= 4 ? fb : fa[j];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[16 * c + i] = fmaf(v[i], c < 4 ? fa : fb, acc[16 * c + i]);
+            for (int i = 0; i < 16; ++i) acc[at + i] = fmaf(v[i], f, acc[at + i]);
           }
-        } else if (lane == 0) {
+        } else {
           d_read(buf);
         }
       }
+      bool whole = true;
+      if (sg.kb1 - sg.kb0 < KBU) {
+        // ---------------- a range of the sum: partial sums [slot][rank][half][4-column group][row], 512 contiguous bytes a store
+        int c0, c1;
+        sched.sharers(sg.item, c0, c1);
+        auto part = [&](int w) {
+          const size_t at = ((size_t)sched.slot(w, sg.item) * group + rank) * 2 + half;
+          return reinterpret_cast<float4*>(p.g.part) + at * (TN / 8) * C::kRows + m;
+        };
+        if (mine) {
+          float4* dst = part(sched.worker);
+#pragma unroll
+          for (int i = 0; i < TN / 8; ++i)
+            __stcg(dst + i * C::kRows, make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]));
+        }
+        __threadfence();
+        int* arrived = p.g.arrived + ((sg.item - sched.first) * group + rank) * 8;
+        if constexpr (SWIGLU) {                            // one decision for the two halves of a row
+          if (!pair_meet(&meet[q], met)) goto late;        // both are written
+          const int at = (met & 1) * 4 + q;
+          if (half == 0 && lane == 0) flag[at] = atomicAdd(&arrived[q], 1) == c1 - c0;
+          if (!pair_meet(&meet[q], met)) goto late;
+          whole = flag[at] != 0;
+        } else {
+          int old = 0;
+          __syncwarp();
+          if (lane == 0) old = atomicAdd(&arrived[4 * half + q], 1);
+          whole = __shfl_sync(0xffffffffu, old, 0) == c1 - c0;
+        }
+        if (whole) __threadfence();
+        // The last worker to arrive adds the tile's ranges in their order, 8 loads under way at once.
+#pragma unroll
+        for (int i = 0; i < TN / 2; ++i) acc[i] = 0.f;
+        if (whole && mine) {
+          for (int w = c0; w <= c1; ++w) {
+            const float4* src = part(w);
+#pragma unroll
+            for (int i = 0; i < TN / 8; i += 8) {
+              float4 v[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v[j] = __ldcg(src + (i + j) * C::kRows);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                acc[4 * (i + j)] += v[j].x;
+                acc[4 * (i + j) + 1] += v[j].y;
+                acc[4 * (i + j) + 2] += v[j].z;
+                acc[4 * (i + j) + 3] += v[j].w;
+              }
+            }
+          }
+        }
+      }
+      // ------------------------------------------------------------------- the whole sum: this thread's row, its columns
       const int rows = p.g.rows;
-      if (sg.kb0 == 0 && sg.kb1 == p.KB) {
-        // ------------------------------------------------------------- the whole sum: this thread's row, 128 columns
+      if (whole) {
         if constexpr (SWIGLU) {
+          static_assert(!SWIGLU || TN == 256, "a row's maximum over 128 columns is taken inside one tile");
           const int col0 = it.nt * 128 + 64 * half;
           float top = 0.f;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float h[2];
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              h[c] = col0 + 2 * i + c < rows
-                         ? swiglu_keep_nan(acc[2 * i + c], acc[64 + 2 * i + c], p.g.limit)
-                         : 0.f;
-              top = max_nan(top, fabsf(h[c]));
-            }
-            acc[2 * i] = h[0];
-            acc[2 * i + 1] = h[1];
+          for (int i = 0; i < 64; ++i) {
+            acc[i] = col0 + i < rows ? swiglu_keep_nan(acc[i], acc[64 + i], p.g.limit) : 0.f;
+            top = max_nan(top, fabsf(acc[i]));
           }
           float* mx = row_max + ((met & 1) * 4 + q) * 64;
           mx[half * 32 + lane] = top;
-          if (!pair_meet(&meet[q], met)) goto done;
+          if (!pair_meet(&meet[q], met)) goto late;
           top = max_nan(top, mx[(half ^ 1) * 32 + lane]);
           float inv;
           const float sc = fp8_group_scale(top, &inv);
@@ -474,141 +592,28 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const Fp8Param
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const int c = 16 * u + 4 * i;
-                w[i] = fp8_pack4(acc[c] * inv, acc[c + 1] * inv, acc[c + 2] * inv,
-                                 acc[c + 3] * inv);
+                w[i] = fp8_pack4(acc[c] * inv, acc[c + 1] * inv, acc[c + 2] * inv, acc[c + 3] * inv);
               }
               dst[u] = make_uint4(w[0], w[1], w[2], w[3]);
             }
             if (half == 0) p.g.hs[xrow * p.hs_ld + it.nt] = sc;
           }
         } else if (mine) {
-          const int col0 = it.nt * 256 + 128 * half;
-          OUT* dst = static_cast<OUT*>(p.g.out) + xrow * rows + col0;
-          constexpr int kU = 32 / (int)sizeof(OUT);        // one 32-byte store: a whole sector of this row
-          if (rows % kU == 0 && (reinterpret_cast<uintptr_t>(p.g.out) & 31) == 0) {
-#pragma unroll
-            for (int u = 0; u < 128 / kU; ++u) {
-              union {
-                uint32_t w[8];
-                OUT o[kU];
-              } b;
-#pragma unroll
-              for (int i = 0; i < kU; ++i) b.o[i] = out_of<OUT>(acc[u * kU + i]);
-              if (col0 + u * kU < rows) store32(dst + u * kU, b.w);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 128; ++i)
-              if (col0 + i < rows) dst[i] = out_of<OUT>(acc[i]);
-          }
-        }
-        continue;
-      }
-      // ----------------------------------------------- a range of the sum: partial sums [slot][rank][half][row][128 columns]
-      int c0, c1;
-      sched.sharers(sg.item, c0, c1);
-      auto part = [&](int w, int row) {
-        const size_t at = ((size_t)sched.slot(w, sg.item) * group + rank) * 2 + half;
-        return reinterpret_cast<float4*>(p.g.part) + (at * C::kRows + row) * 32;
-      };
-      int* arrived = p.g.arrived + ((sg.item - sched.first) * group + rank) * 8;
-      if (mine) {
-        float4* dst = part(sched.worker, m);
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          __stcg(dst + i, make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]));
-      }
-      __threadfence();
-      bool last;
-      if constexpr (SWIGLU) {
-        if (!pair_meet(&meet[q], met)) goto done;          // both halves are written
-        if (half == 0 && lane == 0) {
-          flag[(met & 1) * 4 + q] = atomicAdd(&arrived[q], 1) == c1 - c0;
-          __threadfence();
-        }
-        const int at = (met & 1) * 4 + q;
-        if (!pair_meet(&meet[q], met)) goto done;
-        last = flag[at] != 0;
-      } else {
-        int old = 0;
-        __syncwarp();
-        if (lane == 0) old = atomicAdd(&arrived[4 * half + q], 1);
-        last = __shfl_sync(0xffffffffu, old, 0) == c1 - c0;
-      }
-      if (!last) continue;
-      __threadfence();
-      // The last worker of the tile: lanes take columns now (4 each), rows one after another.
-      const int nr = min(32, it.cnt - 32 * q);
-      // 8 rows at a time, so that 8 loads (16 for two matrices) are under way at once.
-      for (int r0 = 0; r0 < nr; r0 += 8) {
-        float4 sum[8];                       // SwiGLU: gate columns in x, y and up columns in z, w
-#pragma unroll
-        for (int r = 0; r < 8; ++r) sum[r] = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int c = c0; c <= c1; ++c) {
-          const float4* src = part(c, 32 * q + r0);
-#pragma unroll
-          for (int r = 0; r < 8; ++r) {
-            if (r0 + r >= nr) break;
-            float4 a;
-            if constexpr (SWIGLU) {
-              const float2* s2 = reinterpret_cast<const float2*>(src + 32 * r);
-              const float2 g = __ldcg(s2 + lane), u = __ldcg(s2 + 32 + lane);
-              a = make_float4(g.x, g.y, u.x, u.y);
-            } else {
-              a = __ldcg(src + 32 * r + lane);
-            }
-            sum[r].x += a.x;
-            sum[r].y += a.y;
-            sum[r].z += a.z;
-            sum[r].w += a.w;
-          }
-        }
-        if constexpr (SWIGLU) {
-          const int col0 = it.nt * 128 + 64 * half + 2 * lane;
-          float* mx = row_max + ((met & 1) * 4 + q) * 64;
-#pragma unroll
-          for (int r = 0; r < 8; ++r) {
-            sum[r].x = col0 < rows ? swiglu_keep_nan(sum[r].x, sum[r].z, p.g.limit) : 0.f;
-            sum[r].y = col0 + 1 < rows ? swiglu_keep_nan(sum[r].y, sum[r].w, p.g.limit) : 0.f;
-            float top = max_nan(fabsf(sum[r].x), fabsf(sum[r].y));
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, d));
-            if (lane == 0) mx[half * 32 + r] = top;
-          }
-          if (!pair_meet(&meet[q], met)) goto done;
-#pragma unroll
-          for (int r = 0; r < 8; ++r) {
-            if (r0 + r >= nr) break;
-            float inv;
-            const float sc = fp8_group_scale(max_nan(mx[r], mx[32 + r]), &inv);
-            const size_t row = (size_t)it.row0 + 32 * q + r0 + r;
-            *reinterpret_cast<uint16_t*>(p.g.hq + row * ((size_t)p.RB * 128) + col0) = (uint16_t)__nv_cvt_float2_to_fp8x2(
-                make_float2(sum[r].x * inv, sum[r].y * inv), __NV_SATFINITE, __NV_E4M3);
-            if (half == 0 && lane == 0) p.g.hs[row * p.hs_ld + it.nt] = sc;
-          }
-        } else {
-          const int col0 = it.nt * 256 + 128 * half + 4 * lane;
-          const bool wide = rows % 4 == 0 && (reinterpret_cast<uintptr_t>(p.g.out) & 15) == 0;
-#pragma unroll
-          for (int r = 0; r < 8; ++r) {
-            if (r0 + r >= nr) break;
-            struct alignas(4 * sizeof(OUT)) Out4 {
-              OUT o[4];
-            } b = {{out_of<OUT>(sum[r].x), out_of<OUT>(sum[r].y), out_of<OUT>(sum[r].z), out_of<OUT>(sum[r].w)}};
-            OUT* dst = static_cast<OUT*>(p.g.out) + ((size_t)it.row0 + 32 * q + r0 + r) * rows + col0;
-            if (wide) {
-              if (col0 < rows) *reinterpret_cast<Out4*>(dst) = b;
-            } else {
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (col0 + i < rows) dst[i] = b.o[i];
-            }
-          }
+          const int col0 = it.nt * TN + half * (TN / 2);
+          if (p.g.out_type == CBMOE_BF16) store_row<TN / 2, __nv_bfloat16>(p.g.out, xrow, rows, col0, acc);
+          else if (p.g.out_type == CBMOE_F16) store_row<TN / 2, __half>(p.g.out, xrow, rows, col0, acc);
+          else store_row<TN / 2, float>(p.g.out, xrow, rows, col0, acc);
         }
       }
+      sg = sn;
+      it = itn;
+      have = have_n;
     }
   }
-done:
+  if (false) {
+  late:
+    atomicOr(&g_device_errors, CBMOE_DEVERR_TIMEOUT);
+  }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
@@ -634,22 +639,21 @@ int make_fp8_map(CUtensorMap* map, const void* base, int K, long long rows, long
   return r == CUDA_SUCCESS ? CBMOE_OK : CBMOE_ERR_CUDA;
 }
 
-template <int MT, bool SWIGLU, typename OUT>
+template <int MT, int TN, bool SWIGLU>
 int launch_t(const Fp8Gemm& g, cudaStream_t stream) {
-  using C = Fp8Cfg<MT>;
+  using C = Fp8Cfg<MT, TN>;
   Fp8Params p;
   p.g = g;
   p.KB = (g.K + kFp8Group - 1) / kFp8Group;
   p.RB = (g.rows + 127) / 128;
+  p.NT = SWIGLU ? p.RB : (g.rows + TN - 1) / TN;
   p.hs_ld = fp8_scale_stride(g.rows);
-  p.xs_wide = g.ldxs % 4 == 0 && (reinterpret_cast<uintptr_t>(g.xs) & 15) == 0;
-  p.NT = SWIGLU ? p.RB : (p.RB + 1) / 2;
   CUtensorMap mx, m0, m1;
   int rc = make_fp8_map(&mx, g.xq, g.K, g.x_rows, g.ldx, C::kRows);
-  if (!rc) rc = make_fp8_map(&m0, g.w0, g.K, (long long)g.E * g.rows, g.ldw, 128);
-  if (!rc) rc = make_fp8_map(&m1, SWIGLU ? g.w1 : g.w0, g.K, (long long)g.E * g.rows, g.ldw, 128);
+  if (!rc) rc = make_fp8_map(&m0, g.w0, g.K, (long long)g.E * g.rows, g.ldw, TN / 2);
+  if (!rc) rc = make_fp8_map(&m1, SWIGLU ? g.w1 : g.w0, g.K, (long long)g.E * g.rows, g.ldw, TN / 2);
   if (rc) return rc;
-  auto kern = fp8_gemm_kernel<MT, SWIGLU, OUT>;
+  auto kern = fp8_gemm_kernel<MT, TN, SWIGLU>;
   static PerDevice s_attr;
   long long set = 0;
   rc = per_device(s_attr, [&](long long& v) -> int {
@@ -678,12 +682,16 @@ int launch_t(const Fp8Gemm& g, cudaStream_t stream) {
   return CBMOE_OK;
 }
 
+// Weight rows per tile with few tokens, by how many tiles that gives (for experts: at most one pass per slot is counted).
+// Measured on one B200: 5120 -> 12288, 1 token: 48 tiles of 256 25.8 us, 96 of 128 15.5, 192 of 64 19.2; 77 x 5000 -> 1411:
+// 6 of 256 26.8, 12 of 128 20.0, 23 of 64 16.3; the down product of 54 experts, 1080 tiles of 256: 119 us at either width.
 template <int MT>
-int launch_mt(const Fp8Gemm& g, cudaStream_t s) {
-  if (g.w1 != nullptr) return launch_t<MT, true, float>(g, s);
-  if (g.out_type == CBMOE_BF16) return launch_t<MT, false, __nv_bfloat16>(g, s);
-  if (g.out_type == CBMOE_F16) return launch_t<MT, false, __half>(g, s);
-  return launch_t<MT, false, float>(g, s);
+int launch_few(const Fp8Gemm& g, cudaStream_t s) {
+  if (g.w1 != nullptr) return launch_t<MT, 256, true>(g, s);
+  const long long passes = g.pass_expert ? (g.x_rows < g.E ? g.x_rows : g.E) : (g.x_rows + MT - 1) / MT;
+  if (passes * ((g.rows + 255) / 256) >= 2LL * num_sms()) return launch_t<MT, 256, false>(g, s);
+  if (passes * ((g.rows + 127) / 128) >= num_sms() / 2) return launch_t<MT, 128, false>(g, s);
+  return launch_t<MT, 64, false>(g, s);
 }
 
 bool aligned(const void* p, int n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -708,10 +716,11 @@ size_t fp8_part_bytes(int mt) { return (size_t)num_sms() * 2 * (mt < 128 ? mt : 
 int fp8_arrived() { return num_sms() * 8; }
 
 int launch_fp8_gemm(const Fp8Gemm& g, int mt, cudaStream_t s) {
-  if (mt == 32) return launch_mt<32>(g, s);
-  if (mt == 64) return launch_mt<64>(g, s);
-  if (mt == 128) return launch_mt<128>(g, s);
-  return launch_mt<256>(g, s);
+  if (mt == 32) return launch_few<32>(g, s);
+  if (mt == 64) return launch_few<64>(g, s);
+  if (mt == 128) return launch_few<128>(g, s);
+  if (g.w1 != nullptr) return launch_t<256, 256, true>(g, s);
+  return launch_t<256, 256, false>(g, s);
 }
 
 int launch_fp8_quantize(const void* x, int type, int N, int K, long long ldx, uint8_t* q, long long ldq, float* s, int lds,
@@ -741,8 +750,8 @@ int launch_fp8_quantize(const void* x, int type, int N, int K, long long ldx, ui
 
 namespace {
 
-// Workspace of a product: partial sums | counters | q [N][blocks * 128] | s [N][blocks] (the last two where x is quantised
-// here).
+// Workspace of a product: partial sums | counters | q [N][blocks * 128] (where x is quantised here) |
+// scales [N][fp8_scale_stride].
 struct LinearWs {
   size_t arrived, xq, xs, total;
   int mt;
@@ -753,7 +762,7 @@ LinearWs linear_ws(int N, int K, bool ready) {
   w.arrived = lyr::align_up(fp8_part_bytes(w.mt));
   w.xq = w.arrived + lyr::align_up((size_t)fp8_arrived() * 4);
   w.xs = w.xq + (ready ? 0 : lyr::align_up((size_t)N * blocks_of(K) * kFp8Group));
-  w.total = w.xs + (ready ? 0 : lyr::align_up((size_t)N * fp8_scale_stride(K) * 4));
+  w.total = w.xs + lyr::align_up((size_t)N * fp8_scale_stride(K) * 4);
   return w;
 }
 
@@ -835,11 +844,17 @@ extern "C" int cbmoe_fp8_linear(const void* q, long long ldq, const float* s, in
   g.part = reinterpret_cast<float*>(ws);
   g.arrived = reinterpret_cast<int*>(ws + W.arrived);
   if (ready) {
-    CBMOE_CUDA_TRY(cudaMemsetAsync(g.arrived, 0, (size_t)fp8_arrived() * 4, stream));
+    float* sc = reinterpret_cast<float*>(ws + W.xs);
     g.xq = x;
     g.ldx = ldx;
-    g.xs = xs;
-    g.ldxs = blocks_of(K);
+    g.xs = sc;
+    g.ldxs = fp8_scale_stride(K);
+    const long long blocks = ((long long)N * g.ldxs + 255) / 256, cap = num_sms() * 8;
+    prof_begin(kProfOther, stream);
+    CBMOE_CUDA_TRY(launch_pdl(fp8_scales_kernel, dim3((int)(blocks < cap ? blocks : cap)), dim3(256), 0, stream, xs, N,
+                              blocks_of(K), g.ldxs, sc, g.arrived, fp8_arrived()));
+    prof_end(kProfOther, stream);
+    CBMOE_CUDA_TRY(cudaGetLastError());
   } else {
     float* sc = reinterpret_cast<float*>(ws + W.xs);
     g.ldxs = fp8_scale_stride(K);

@@ -45,7 +45,7 @@ struct Fp8Gemm {
   const void* xq;          // e4m3 [x_rows][ldx]
   long long ldx;
   int x_rows;
-  const float* xs;         // [x_rows][ldxs], ldxs >= ceil(K / 128)
+  const float* xs;         // [x_rows][ldxs], ldxs = fp8_scale_stride(K), 16-byte aligned
   int ldxs;
   const void* w0;          // e4m3 [E][rows][ldw]; w1: up, beside w0 = gate (SwiGLU), else null
   const void* w1;
