@@ -1,5 +1,6 @@
 """ctypes binding of libcbmoe.so (include/cbmoe.h). The library is required: there is no CPU fallback, and every
 function here raises if the library or a CUDA device is missing."""
+import contextlib
 import ctypes
 import os
 
@@ -153,12 +154,28 @@ def stream_handle(device=None):
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def raw_stream(t):
+    """The current stream of t's device as a plain handle."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
 def require_cuda(*tensors):
-    if not torch.cuda.is_available():
-        raise CbmoeError("cbmoe needs a CUDA device (no CPU fallback)")
     for t in tensors:
         if t is not None and not t.is_cuda:
+            if not torch.cuda.is_available():
+                break
             raise CbmoeError("cbmoe tensors must live on the GPU")
+    else:
+        return
+    raise CbmoeError("cbmoe needs a CUDA device (no CPU fallback)")
+
+
+_same_device = contextlib.nullcontext()
+
+
+def on_device(t):
+    """Context with t's device current (costs nothing when it is already)."""
+    return _same_device if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
 
 
 def device_errors(clear=True):

@@ -10,7 +10,7 @@ Activations are quantised per row in groups of 128 (ops.fp8_quantize); so is the
 import torch
 
 from . import ops
-from ._lib import TYPES, Fp8Experts, check, lib, ptr, require_cuda, stream_handle
+from ._lib import TYPES, Fp8Experts, check, lib, on_device, raw_stream, require_cuda
 
 FP8 = "FP8"
 
@@ -48,11 +48,12 @@ def apply(p, x, idx, w, limit, out_dtype=torch.float32):
     if p["gate_q"][0].device != x.device:
         raise ValueError(f"tables on {p['gate_q'][0].device}, x on {x.device}")
     ex = experts_struct(p)
-    with torch.cuda.device(x.device):
+    with on_device(x):
         y = torch.empty((N, p["H"]), dtype=out_dtype, device=x.device)
         # per call, from the caching allocator: calls on several streams and captured graphs share nothing
         nbytes = lib().cbmoe_fp8_experts_workspace_bytes(ex, N, k, TYPES[out_dtype])
         ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=x.device)
-        check(lib().cbmoe_fp8_experts_apply(ex, ptr(x), N, ptr(idx), ptr(w), k, float(limit), ptr(y), TYPES[out_dtype],
-                                            ptr(ws), nbytes, stream_handle()), "cbmoe_fp8_experts_apply")
+        check(lib().cbmoe_fp8_experts_apply(ex, x.data_ptr(), N, idx.data_ptr(), w.data_ptr(), k, float(limit),
+                                            y.data_ptr(), TYPES[out_dtype], ws.data_ptr(), nbytes, raw_stream(x)),
+              "cbmoe_fp8_experts_apply")
     return y

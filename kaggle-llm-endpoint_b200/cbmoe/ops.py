@@ -7,7 +7,7 @@ import ctypes
 
 import torch
 
-from ._lib import E4M3, TYPES, check, lib, ptr, require_cuda, stream_handle
+from ._lib import E4M3, TYPES, check, lib, on_device, ptr, raw_stream, require_cuda, stream_handle
 
 PLAN_FIELDS = ("counts", "row_start", "act", "n_act", "n_blocks", "n_pass", "blk_expert", "tok_row", "w_row",
                "row_slot", "pass_expert", "pass_row0", "pass_cnt")
@@ -103,22 +103,16 @@ def route_plan(idx, w, E, tm, pass_tokens=8):
     buf = torch.empty(off[13], dtype=torch.int32, device=idx.device)
     check(lib().cbmoe_route_plan(ptr(_contig(idx, torch.int32)), ptr(_contig(w, torch.float32)), T, k, E, tm,
                                  pass_tokens, ptr(buf), off[13] * 4, stream_handle()), "cbmoe_route_plan")
-    out = {}
-    for i, name in enumerate(PLAN_FIELDS):
-        v = buf[off[i]:off[i + 1]] if i < 12 else buf[off[i]:off[13]]
-        out[name] = v
-    for name, n in (("counts", E), ("row_start", E), ("act", E)):
-        out[name] = out[name][:n]
-    out["n_act"], out["n_blocks"], out["n_pass"] = out["n_act"][:1], out["n_blocks"][:1], out["n_pass"][:1]
     S = T * k
     G = -(-S // tm) + E
     P = -(-S // pass_tokens) + E
-    out["blk_expert"] = out["blk_expert"][:G]
-    out["tok_row"] = out["tok_row"][:G * tm]
-    out["w_row"] = out["w_row"][:G * tm].view(torch.float32)
-    out["row_slot"] = out["row_slot"][:S].view(T, k)
-    for name in ("pass_expert", "pass_row0", "pass_cnt"):
-        out[name] = out[name][:P]
+    used = (E, E, E, 1, 1, 1, G, G * tm, G * tm, S, P, P, P)
+    sizes = []
+    for i, n in enumerate(used):   # each field and what pads it to the next one: one split instead of a view per field
+        sizes += [n, off[i + 1] - off[i] - n]
+    out = dict(zip(PLAN_FIELDS, buf.split(sizes)[::2]))
+    out["w_row"] = out["w_row"].view(torch.float32)
+    out["row_slot"] = out["row_slot"].view(T, k)
     return out
 
 
@@ -179,10 +173,10 @@ def fp8_quantize(x):
     if K == 0:
         raise ValueError("x has no columns")
     ld = -(-K // 16) * 16
-    with torch.cuda.device(x.device):
+    with on_device(x):
         q = torch.empty((N, ld), dtype=torch.float8_e4m3fn, device=x.device)
         s = torch.empty((N, -(-K // 128)), dtype=torch.float32, device=x.device)
-        check(lib().cbmoe_fp8_quantize(ptr(x), TYPES[x.dtype], N, K, ldx, ptr(q), ld, ptr(s), stream_handle()),
+        check(lib().cbmoe_fp8_quantize(x.data_ptr(), TYPES[x.dtype], N, K, ldx, q.data_ptr(), ld, s.data_ptr(), raw_stream(x)),
               "cbmoe_fp8_quantize")
     return q[:, :K], s
 
@@ -253,10 +247,11 @@ def fp8_linear(q, s, x, out_dtype=torch.float32):
             raise ValueError(f"x is bf16, fp16 or fp32, got {xv.dtype}")
         xv, ldx = _fp8_x(xv)
         code = TYPES[xv.dtype]
-    with torch.cuda.device(xv.device):
+    with on_device(xv):
         y = torch.empty((N, rows), dtype=out_dtype, device=xv.device)
         nbytes = lib().cbmoe_fp8_linear_workspace_bytes(N, K, rows, code)
         ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=xv.device)
-        check(lib().cbmoe_fp8_linear(ptr(q), ldq, ptr(s), rows, K, ptr(xv), code, ldx, ptr(xs), N, ptr(y),
-                                     TYPES[out_dtype], ptr(ws), nbytes, stream_handle()), "cbmoe_fp8_linear")
+        check(lib().cbmoe_fp8_linear(q.data_ptr(), ldq, s.data_ptr(), rows, K, xv.data_ptr(), code, ldx,
+                                     None if xs is None else xs.data_ptr(), N, y.data_ptr(), TYPES[out_dtype],
+                                     ws.data_ptr(), nbytes, raw_stream(xv)), "cbmoe_fp8_linear")
     return y

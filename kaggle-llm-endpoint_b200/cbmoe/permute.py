@@ -11,21 +11,24 @@ backward give the same bits on every call.
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._lib import TYPES, check, lib, ptr, require_cuda, stream_handle
+from ._lib import TYPES, check, lib, on_device, raw_stream, require_cuda
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _plan_rows(plan, device):
     """(tok_row [R], row_slot [T, k]) of a plan; with blocks of one row the R = T k rows that can be in use."""
     tok_row, row_slot = plan["tok_row"], plan["row_slot"]
     for name, t, dim in (("tok_row", tok_row, 1), ("row_slot", row_slot, 2)):
-        if t.dtype != torch.int32 or t.dim() != dim or not t.is_contiguous():
-            raise ValueError(f"plan[{name!r}] is contiguous int32 of {dim} dimension(s), got {t.dtype} {tuple(t.shape)}")
-        if t.device != device:
-            raise ValueError(f"plan[{name!r}] is on {t.device}, the rows on {device}")
+        if t.dtype is not torch.int32 or t.dim() != dim or not t.is_contiguous() or t.device != device:
+            raise ValueError(f"plan[{name!r}] is contiguous int32 of {dim} dimension(s) on {device}, got {t.dtype} "
+                             f"{tuple(t.shape)} on {t.device}")
     if row_slot.shape[1] == 0:
         raise ValueError("the plan has no slots per token")
     blocks = plan.get("blk_expert")
-    if blocks is not None and blocks.numel() == tok_row.numel():
+    if blocks is not None and blocks.shape[0] == tok_row.shape[0]:
         tok_row = tok_row[:row_slot.numel()]
     return tok_row, row_slot
 
@@ -41,18 +44,18 @@ def _rows(name, t):
 def _permute(x, tok_row, row_slot):
     (T, k), R, H = row_slot.shape, tok_row.numel(), x.shape[1]
     xs = torch.empty((R, H), dtype=x.dtype, device=x.device)
-    with torch.cuda.device(x.device):
-        check(lib().cbmoe_permute(ptr(x), TYPES[x.dtype], T, H, ptr(row_slot), k, ptr(tok_row), R, ptr(xs),
-                                  stream_handle()), "cbmoe_permute")
+    with on_device(x):
+        check(lib().cbmoe_permute(x.data_ptr(), TYPES[x.dtype], T, H, row_slot.data_ptr(), k, tok_row.data_ptr(), R,
+                                  xs.data_ptr(), raw_stream(row_slot)), "cbmoe_permute")
     return xs
 
 
 def _unpermute(ys, w, row_slot):
     (T, k), (R, H) = row_slot.shape, ys.shape
     y = torch.empty((T, H), dtype=ys.dtype, device=ys.device)
-    with torch.cuda.device(ys.device):
-        check(lib().cbmoe_unpermute(ptr(ys), TYPES[ys.dtype], R, H, ptr(row_slot), ptr(w), T, k, ptr(y),
-                                    stream_handle()), "cbmoe_unpermute")
+    with on_device(ys):
+        check(lib().cbmoe_unpermute(ys.data_ptr(), TYPES[ys.dtype], R, H, row_slot.data_ptr(), _ptr(w), T, k,
+                                    y.data_ptr(), raw_stream(row_slot)), "cbmoe_unpermute")
     return y
 
 
@@ -86,10 +89,10 @@ class _Unpermute(torch.autograd.Function):
         need_ys, need_w = ctx.needs_input_grad[:2]
         dys = torch.empty((R, H), dtype=dy.dtype, device=dy.device) if need_ys else None
         dw = torch.empty((T, k), dtype=torch.float32, device=dy.device) if need_w else None
-        with torch.cuda.device(dy.device):
-            check(lib().cbmoe_unpermute_backward(ptr(dy), ptr(ys), TYPES[dy.dtype], R, H, ptr(row_slot), ptr(tok_row),
-                                                 ptr(w), T, k, ptr(dys), ptr(dw), stream_handle()),
-                  "cbmoe_unpermute_backward")
+        with on_device(dy):
+            check(lib().cbmoe_unpermute_backward(dy.data_ptr(), _ptr(ys), TYPES[dy.dtype], R, H, row_slot.data_ptr(),
+                                                 tok_row.data_ptr(), w.data_ptr(), T, k, _ptr(dys), _ptr(dw),
+                                                 raw_stream(row_slot)), "cbmoe_unpermute_backward")
         return dys, dw, None, None
 
 

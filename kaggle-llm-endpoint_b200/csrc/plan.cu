@@ -262,9 +262,18 @@ __device__ __forceinline__ void chunk_warp_counts(const int32_t* idx, int beg, i
   }
 }
 
+// Also sets every sorted row to padding (the placement overwrites the rows in use).
 __global__ void __launch_bounds__(kPlanCtaWarps * 32) plan_count_kernel(const int32_t* __restrict__ idx, int S, int E,
+                                                                        int32_t* __restrict__ plan, PlanLayout L,
                                                                         int32_t* __restrict__ chunk_cnt) {
   extern __shared__ int cnt[];  // [kPlanCtaWarps][E]
+  const int Rp = (int)(L.off[8] - L.off[7]);
+  int32_t* tok_row = plan + L.off[7];
+  float* w_row = reinterpret_cast<float*>(plan + L.off[8]);
+  for (int r = blockIdx.x * blockDim.x + threadIdx.x; r < Rp; r += gridDim.x * blockDim.x) {
+    tok_row[r] = -1;
+    w_row[r] = 0.f;
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int c0 = blockIdx.x * kPlanChunkSlots;
   const int per = kPlanChunkSlots / kPlanCtaWarps;
@@ -285,8 +294,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_scan_kernel(int T, int k, i
                                                                  int* __restrict__ zero, int n_zero) {
   extern __shared__ int sm[];
   int* counts = sm;        // [E]
-  int* ends = sm + E;      // [E]
-  int* bases = sm + 2 * E; // [E] first sorted row of each expert
+  int* bases = sm + E;     // [E] first sorted row of each expert
   __shared__ int s_tot[4];
   __shared__ int s_chunk[4][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -339,11 +347,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_scan_kernel(int T, int k, i
     }
   }
   __syncthreads();
-  int c_rows, c_blocks, c_pass, c_act, tot_rows, tot_blocks, tot_pass, tot_act;
+  int c_rows, c_pass, c_act, tot_rows, tot_blocks, tot_pass, tot_act;
   {
     const bool in = lane < n_ech;
     c_rows = warp_exclusive_scan(in ? s_chunk[0][lane] : 0, &tot_rows);
-    c_blocks = warp_exclusive_scan(in ? s_chunk[1][lane] : 0, &tot_blocks);
+    warp_exclusive_scan(in ? s_chunk[1][lane] : 0, &tot_blocks);
     c_pass = warp_exclusive_scan(in ? s_chunk[2][lane] : 0, &tot_pass);
     c_act = warp_exclusive_scan(in ? s_chunk[3][lane] : 0, &tot_act);
   }
@@ -354,13 +362,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_scan_kernel(int T, int k, i
     const int np = (c + pass_tokens - 1) / pass_tokens;
     int dummy;
     const int x_rows = warp_exclusive_scan(nb * tm, &dummy) + __shfl_sync(0xffffffffu, c_rows, q);
-    const int x_blocks = warp_exclusive_scan(nb, &dummy) + __shfl_sync(0xffffffffu, c_blocks, q);
     const int x_pass = warp_exclusive_scan(np, &dummy) + __shfl_sync(0xffffffffu, c_pass, q);
     const int x_act = warp_exclusive_scan(c > 0 ? 1 : 0, &dummy) + __shfl_sync(0xffffffffu, c_act, q);
     if (e < E) {
       counts_g[e] = c;
       row_start[e] = x_rows;
-      ends[e] = x_blocks + nb;
       if (c > 0) act[x_act] = e;
       for (int p = 0; p < np; ++p) {
         pass_expert[x_pass + p] = e;
@@ -384,13 +390,6 @@ __global__ void __launch_bounds__(kPlanThreads) plan_scan_kernel(int T, int k, i
     plan[L.off[4]] = tot_blocks;
     plan[L.off[5]] = tot_pass;
   }
-  const int Rp = (int)(L.off[8] - L.off[7]);
-  int32_t* tok_row = plan + L.off[7];
-  float* w_row = reinterpret_cast<float*>(plan + L.off[8]);
-  for (int r = threadIdx.x; r < Rp; r += kPlanThreads) {
-    tok_row[r] = -1;
-    w_row[r] = 0.f;
-  }
   __syncthreads();
   for (int i = s_tot[0] + threadIdx.x; i < E; i += kPlanThreads) act[i] = -1;
   for (int i = s_tot[2] + threadIdx.x; i < P; i += kPlanThreads) {
@@ -398,26 +397,32 @@ __global__ void __launch_bounds__(kPlanThreads) plan_scan_kernel(int T, int k, i
     pass_row0[i] = 0;
     pass_cnt[i] = 0;
   }
-  const int G = (int)(L.off[7] - L.off[6]);
-  int32_t* blk_expert = plan + L.off[6];
-  const int n_blocks = s_tot[1];
-  auto find = [&](int g) {
-    int lo = 0, hi = E;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (ends[mid] > g) hi = mid; else lo = mid + 1;
-    }
-    return min(lo, E - 1);
-  };
-  const int last = find(max(n_blocks - 1, 0));
-  for (int g = threadIdx.x; g < G; g += kPlanThreads) blk_expert[g] = (g < n_blocks) ? find(g) : last;
 }
 
 __global__ void __launch_bounds__(kPlanCtaWarps * 32) plan_place_kernel(const int32_t* __restrict__ idx,
                                                                         const float* __restrict__ wts, int S, int k,
-                                                                        int E, int32_t* __restrict__ plan, PlanLayout L,
+                                                                        int E, int tm, int32_t* __restrict__ plan,
+                                                                        PlanLayout L,
                                                                         const int32_t* __restrict__ chunk_base) {
   extern __shared__ int cnt[];  // [kPlanCtaWarps][E]
+  // block -> expert for this CTA's share of the blocks: the first expert whose block range ends after the block; blocks
+  // past n_blocks repeat the last (cnt[0, E): the ends)
+  const int32_t* counts_g = plan + L.off[0];
+  const int32_t* row_start = plan + L.off[1];
+  for (int e = threadIdx.x; e < E; e += blockDim.x) cnt[e] = row_start[e] / tm + (counts_g[e] + tm - 1) / tm;
+  __syncthreads();
+  const int G = (int)(L.off[7] - L.off[6]), n_blocks = plan[L.off[4]];
+  int32_t* blk_expert = plan + L.off[6];
+  for (int g = blockIdx.x * blockDim.x + threadIdx.x; g < G; g += gridDim.x * blockDim.x) {
+    const int at = min(g, max(n_blocks - 1, 0));
+    int lo = 0, hi = E;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (cnt[mid] > at) hi = mid; else lo = mid + 1;
+    }
+    blk_expert[g] = min(lo, E - 1);
+  }
+  __syncthreads();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int c0 = blockIdx.x * kPlanChunkSlots;
   const int per = kPlanChunkSlots / kPlanCtaWarps;
@@ -490,10 +495,10 @@ int launch_route_plan(const int32_t* idx, const float* w, int T, int k, int E, i
     int32_t* chunk = plan + L.off[12] + ((L.off[11] - L.off[10] + 3) & ~3);   // scratch after the pass lists
     const size_t csmem = (size_t)kPlanCtaWarps * E * 4;
     prof_begin(kProfPlan, stream);
-    plan_count_kernel<<<n_chunks, kPlanCtaWarps * 32, csmem, stream>>>(idx, (int)S, E, chunk);
-    plan_scan_kernel<<<1, kPlanThreads, 3 * E * 4, stream>>>(T, k, E, tm, pass_tokens, n_chunks, plan, L, chunk, zero,
+    plan_count_kernel<<<n_chunks, kPlanCtaWarps * 32, csmem, stream>>>(idx, (int)S, E, plan, L, chunk);
+    plan_scan_kernel<<<1, kPlanThreads, 2 * E * 4, stream>>>(T, k, E, tm, pass_tokens, n_chunks, plan, L, chunk, zero,
                                                              n_zero);
-    plan_place_kernel<<<n_chunks, kPlanCtaWarps * 32, csmem, stream>>>(idx, w, (int)S, k, E, plan, L, chunk);
+    plan_place_kernel<<<n_chunks, kPlanCtaWarps * 32, csmem, stream>>>(idx, w, (int)S, k, E, tm, plan, L, chunk);
     prof_end(kProfPlan, stream);
     prof_add_launches(2);
     CBMOE_CUDA_TRY(cudaGetLastError());
