@@ -17,7 +17,7 @@ namespace cbmoe {
 
 namespace {
 
-constexpr int kPermThreads = 256;
+constexpr int kPermThreads = 128;
 
 template <typename T>
 struct Elem;
@@ -44,14 +44,16 @@ struct alignas(VB) Vec {
   T v[n];
 };
 
-// Zero rows of `out` where tok_row < 0: a warp looks at 32 rows at a time.
+// Zero rows of `out` where tok_row < 0: a warp looks at up to 32 rows at a time, at fewer where there are enough warps
+// (a row of padding is a warp's work: 528 rows of 1411 halfs by 17 warps took 15 us).
 template <typename V>
 __device__ __forceinline__ void zero_padding(V* out, const int32_t* __restrict__ tok_row, int R, int HV, int warp0,
                                              int n_warps) {
   const int lane = threadIdx.x & 31;
-  for (long long base = 32LL * warp0; base < R; base += 32LL * n_warps) {
+  const int step = min(32, (R + n_warps - 1) / n_warps);
+  for (long long base = (long long)step * warp0; base < R; base += (long long)step * n_warps) {
     const int r = (int)base + lane;
-    unsigned todo = __ballot_sync(0xffffffffu, r < R && tok_row[r < R ? r : R - 1] < 0);
+    unsigned todo = __ballot_sync(0xffffffffu, lane < step && r < R && tok_row[r < R ? r : R - 1] < 0);
     while (todo) {
       const int row = (int)base + __ffs(todo) - 1;
       todo &= todo - 1;
@@ -61,11 +63,12 @@ __device__ __forceinline__ void zero_padding(V* out, const int32_t* __restrict__
   }
 }
 
+// A token's k rows are looked up once by the threads that copy or sum it: `tpt` threads a token (32 for narrow rows).
 template <typename T, int VB>
 __global__ void __launch_bounds__(kPermThreads) permute_kernel(const Vec<T, VB>* __restrict__ x, int Tn, int HV,
                                                                const int32_t* __restrict__ row_slot, int k,
                                                                const int32_t* __restrict__ tok_row, int R,
-                                                               Vec<T, VB>* __restrict__ xs, int tok_blocks) {
+                                                               Vec<T, VB>* __restrict__ xs, int tok_blocks, int tpt) {
   griddep_wait();
   griddep_launch();
   if ((int)blockIdx.x >= tok_blocks) {
@@ -73,14 +76,21 @@ __global__ void __launch_bounds__(kPermThreads) permute_kernel(const Vec<T, VB>*
                  ((int)gridDim.x - tok_blocks) * (kPermThreads / 32));
     return;
   }
-  const long long total = (long long)Tn * HV;
-  for (long long i = blockIdx.x * (long long)kPermThreads + threadIdx.x; i < total;
-       i += (long long)tok_blocks * kPermThreads) {
-    const int t = (int)(i / HV), c = (int)(i - (long long)t * HV);
-    const Vec<T, VB> v = x[i];
-    for (int j = 0; j < k; ++j) {
-      const int r = row_slot[(size_t)t * k + j];
-      if (r >= 0 && r < R) xs[(size_t)r * HV + c] = v;
+  const int per = kPermThreads / tpt, c0 = threadIdx.x % tpt;
+  for (int t = blockIdx.x * per + threadIdx.x / tpt; t < Tn; t += tok_blocks * per) {
+    for (int j0 = 0; j0 < k; j0 += 8) {
+      int r[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        r[j] = j0 + j < k ? row_slot[(size_t)t * k + j0 + j] : -1;
+        if (r[j] >= R) r[j] = -1;
+      }
+      for (int c = c0; c < HV; c += tpt) {
+        const Vec<T, VB> v = x[(size_t)t * HV + c];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (r[j] >= 0) xs[(size_t)r[j] * HV + c] = v;
+      }
     }
   }
 }
@@ -89,37 +99,37 @@ template <typename T, int VB>
 __global__ void __launch_bounds__(kPermThreads) unpermute_kernel(const Vec<T, VB>* __restrict__ ys, int R, int HV,
                                                                  const int32_t* __restrict__ row_slot,
                                                                  const float* __restrict__ w, int Tn, int k,
-                                                                 Vec<T, VB>* __restrict__ y) {
+                                                                 Vec<T, VB>* __restrict__ y, int tpt) {
   using V = Vec<T, VB>;
   griddep_wait();
   griddep_launch();
-  const long long total = (long long)Tn * HV;
-  for (long long i = blockIdx.x * (long long)kPermThreads + threadIdx.x; i < total;
-       i += (long long)gridDim.x * kPermThreads) {
-    const int t = (int)(i / HV), c = (int)(i - (long long)t * HV);
-    float acc[V::n] = {};
-    for (int j0 = 0; j0 < k; j0 += 8) {   // 8 rows in flight
-      V v[8];
-      float wt[8];
-      bool in[8];
+  const int per = kPermThreads / tpt, c0 = threadIdx.x % tpt;
+  for (int t = blockIdx.x * per + threadIdx.x / tpt; t < Tn; t += gridDim.x * per) {
+    for (int c = c0; c < HV; c += tpt) {
+      float acc[V::n] = {};
+      for (int j0 = 0; j0 < k; j0 += 8) {   // 8 rows in flight
+        V v[8];
+        float wt[8];
+        bool in[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int r = j0 + j < k ? row_slot[(size_t)t * k + j0 + j] : -1;
-        in[j] = r >= 0 && r < R;
-        wt[j] = in[j] && w != nullptr ? w[(size_t)t * k + j0 + j] : 1.f;
-        if (in[j]) v[j] = ys[(size_t)r * HV + c];
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (in[j]) {
-#pragma unroll
-          for (int q = 0; q < V::n; ++q) acc[q] = fmaf(wt[j], Elem<T>::to(v[j].v[q]), acc[q]);
+        for (int j = 0; j < 8; ++j) {
+          const int r = j0 + j < k ? row_slot[(size_t)t * k + j0 + j] : -1;
+          in[j] = r >= 0 && r < R;
+          wt[j] = in[j] && w != nullptr ? w[(size_t)t * k + j0 + j] : 1.f;
+          if (in[j]) v[j] = ys[(size_t)r * HV + c];
         }
-    }
-    V o;
 #pragma unroll
-    for (int q = 0; q < V::n; ++q) o.v[q] = Elem<T>::from(acc[q]);
-    y[i] = o;
+        for (int j = 0; j < 8; ++j)
+          if (in[j]) {
+#pragma unroll
+            for (int q = 0; q < V::n; ++q) acc[q] = fmaf(wt[j], Elem<T>::to(v[j].v[q]), acc[q]);
+          }
+      }
+      V o;
+#pragma unroll
+      for (int q = 0; q < V::n; ++q) o.v[q] = Elem<T>::from(acc[q]);
+      y[(size_t)t * HV + c] = o;
+    }
   }
 }
 
@@ -196,9 +206,10 @@ int blocks_for(long long total, int threads, int per_sm) {
   return (int)(b < 1 ? 1 : (b > cap ? cap : b));
 }
 
-// Blocks beside the token blocks that clear padding rows (each warp checks 32 rows at a time).
+// Threads that share a token, and blocks beside the token blocks that clear padding rows.
+int threads_per_token(int HV) { return HV <= 64 ? 32 : (HV <= 256 ? 64 : 128); }
 int pad_blocks(int R, int threads) {
-  const long long b = ((long long)R + threads - 1) / threads, cap = num_sms();
+  const long long b = ((long long)R * 32 + threads - 1) / threads, cap = num_sms();
   return (int)(b > cap ? cap : b);
 }
 
@@ -213,9 +224,9 @@ template <typename T, int VB>
 int permute_t(const void* x, int Tn, int H, const int32_t* row_slot, int k, const int32_t* tok_row, int R, void* xs,
               cudaStream_t s) {
   using V = Vec<T, VB>;
-  const int HV = H / V::n, tb = blocks_for((long long)Tn * HV, kPermThreads, 32);
+  const int HV = H / V::n, tpt = threads_per_token(HV), tb = blocks_for(Tn, kPermThreads / tpt, 64);
   CBMOE_CUDA_TRY(launch_pdl(permute_kernel<T, VB>, dim3(tb + pad_blocks(R, kPermThreads)), dim3(kPermThreads), 0, s,
-                            static_cast<const V*>(x), Tn, HV, row_slot, k, tok_row, R, static_cast<V*>(xs), tb));
+                            static_cast<const V*>(x), Tn, HV, row_slot, k, tok_row, R, static_cast<V*>(xs), tb, tpt));
   return CBMOE_OK;
 }
 
@@ -224,9 +235,9 @@ int unpermute_t(const void* ys, int R, int H, const int32_t* row_slot, const flo
                 cudaStream_t s) {
   using V = Vec<T, VB>;
   const int HV = H / V::n;
-  CBMOE_CUDA_TRY(launch_pdl(unpermute_kernel<T, VB>, dim3(blocks_for((long long)Tn * HV, kPermThreads, 32)),
-                            dim3(kPermThreads), 0, s, static_cast<const V*>(ys), R, HV, row_slot, w, Tn, k,
-                            static_cast<V*>(y)));
+  const int tpt = threads_per_token(HV);
+  CBMOE_CUDA_TRY(launch_pdl(unpermute_kernel<T, VB>, dim3(blocks_for(Tn, kPermThreads / tpt, 64)), dim3(kPermThreads), 0,
+                            s, static_cast<const V*>(ys), R, HV, row_slot, w, Tn, k, static_cast<V*>(y), tpt));
   return CBMOE_OK;
 }
 
