@@ -236,7 +236,8 @@ int cbmoe_route(const uint16_t* x, int N, int D, const uint16_t* router_w, const
  * multiple of 16, >= K) is an argument, the first row 16-byte aligned, the scales dense. Activations are quantised per
  * row in groups of 128 columns: scale = the least power of two s >= 2^-100 with max|x| <= 448 s, codes = e4m3(x / s)
  * (an exact division; round to nearest even); a group that holds an infinity or a NaN has the scale NaN and stands for
- * NaN, so the row's products are NaN. Any rows >= 1 and K >= 1: sizes need not be multiples of anything.
+ * NaN, so the row's products are NaN. Any rows >= 1 and K >= 1 (products: K <= 2^24, N <= 2^30): sizes need not be multiples of
+ * anything.
  * No counterpart in the reference, which converts such weights to other formats at load time. */
 /* x [N][K] of `type` (CBMOE_BF16 / F16 / F32; row stride ldx elements) -> q [N][K] e4m3 (row stride ldq bytes; bytes
  * between K and ldq may be written with zeros) and s fp32 [N][ceil(K/128)]. */

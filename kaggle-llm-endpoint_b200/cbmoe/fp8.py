@@ -45,8 +45,8 @@ def apply(p, x, idx, w, limit, out_dtype=torch.float32):
     N, k = idx.shape
     if out_dtype not in TYPES:
         raise ValueError(f"out_dtype is fp32, bf16 or fp16, got {out_dtype}")
-    if p["gate_q"][0].device != x.device:
-        raise ValueError(f"tables on {p['gate_q'][0].device}, x on {x.device}")
+    if not p["gate_q"][0].device == x.device == idx.device == w.device:
+        raise ValueError(f"tables on {p['gate_q'][0].device}, x on {x.device}, idx on {idx.device}, w on {w.device}")
     ex = experts_struct(p)
     with on_device(x):
         y = torch.empty((N, p["H"]), dtype=out_dtype, device=x.device)

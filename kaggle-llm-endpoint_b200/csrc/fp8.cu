@@ -791,7 +791,7 @@ ExpertsWs experts_ws(int E, int H, int I, int N, int k, int y_type) {
 }
 
 bool fp8_table_ok(const void* q, const float* s, long long ld, long long rows, int K) {
-  return q && s && aligned(q, 16) && aligned(s, 4) && ld >= K && ld % 16 == 0 && rows <= 0x7fffffffLL;
+  return q && s && aligned(q, 16) && aligned(s, 4) && ld >= K && ld % 16 == 0 && rows <= 0x7ffffe00LL;   // row coordinates of a tile's end in 32 bits
 }
 
 bool fp8_experts_ok(const cbmoe_fp8_experts* ex) {
@@ -827,6 +827,7 @@ extern "C" int cbmoe_fp8_linear(const void* q, long long ldq, const float* s, in
   const bool ready = x_type == CBMOE_E4M3;
   if (!ready && !type_ok(x_type)) return CBMOE_ERR_INVALID;
   if (N == 0) return CBMOE_OK;
+  if (N > (1 << 30) || K > (1 << 24)) return CBMOE_ERR_UNSUPPORTED;   // counts of tiles and blocks in 32 bits
   if (!x || !y || ldx < K || (ready && (!xs || ldx % 16 || !aligned(x, 16)))) return CBMOE_ERR_INVALID;
   Fp8Gemm g{};
   g.rows = rows;

@@ -72,11 +72,12 @@ __global__ void __launch_bounds__(kPermThreads) permute_kernel(const Vec<T, VB>*
   griddep_wait();
   griddep_launch();
   if ((int)blockIdx.x >= tok_blocks) {
-    zero_padding(xs, tok_row, R, HV, ((int)blockIdx.x - tok_blocks) * (kPermThreads / 32) + (threadIdx.x >> 5),
-                 ((int)gridDim.x - tok_blocks) * (kPermThreads / 32));
+    if (blockIdx.y == 0)
+      zero_padding(xs, tok_row, R, HV, ((int)blockIdx.x - tok_blocks) * (kPermThreads / 32) + (threadIdx.x >> 5),
+                   ((int)gridDim.x - tok_blocks) * (kPermThreads / 32));
     return;
   }
-  const int per = kPermThreads / tpt, c0 = threadIdx.x % tpt;
+  const int per = kPermThreads / tpt, c0 = threadIdx.x % tpt + tpt * blockIdx.y, dc = tpt * gridDim.y;
   for (int t = blockIdx.x * per + threadIdx.x / tpt; t < Tn; t += tok_blocks * per) {
     for (int j0 = 0; j0 < k; j0 += 8) {
       int r[8];
@@ -85,7 +86,7 @@ __global__ void __launch_bounds__(kPermThreads) permute_kernel(const Vec<T, VB>*
         r[j] = j0 + j < k ? row_slot[(size_t)t * k + j0 + j] : -1;
         if (r[j] >= R) r[j] = -1;
       }
-      for (int c = c0; c < HV; c += tpt) {
+      for (int c = c0; c < HV; c += dc) {
         const Vec<T, VB> v = x[(size_t)t * HV + c];
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -103,9 +104,9 @@ __global__ void __launch_bounds__(kPermThreads) unpermute_kernel(const Vec<T, VB
   using V = Vec<T, VB>;
   griddep_wait();
   griddep_launch();
-  const int per = kPermThreads / tpt, c0 = threadIdx.x % tpt;
+  const int per = kPermThreads / tpt, c0 = threadIdx.x % tpt + tpt * blockIdx.y, dc = tpt * gridDim.y;
   for (int t = blockIdx.x * per + threadIdx.x / tpt; t < Tn; t += gridDim.x * per) {
-    for (int c = c0; c < HV; c += tpt) {
+    for (int c = c0; c < HV; c += dc) {
       float acc[V::n] = {};
       for (int j0 = 0; j0 < k; j0 += 8) {   // 8 rows in flight
         V v[8];
@@ -208,6 +209,11 @@ int blocks_for(long long total, int threads, int per_sm) {
 
 // Threads that share a token, and blocks beside the token blocks that clear padding rows.
 int threads_per_token(int HV) { return HV <= 64 ? 32 : (HV <= 256 ? 64 : 128); }
+// Blocks along a row where the tokens alone do not fill the GPU (a single token: its columns over as many SMs).
+int row_blocks(int HV, int tpt, int tok_blocks) {
+  const int want = 2 * num_sms() / tok_blocks, most = (HV + tpt - 1) / tpt;
+  return want < 1 ? 1 : (want < most ? want : most);
+}
 int pad_blocks(int R, int threads) {
   const long long b = ((long long)R * 32 + threads - 1) / threads, cap = num_sms();
   return (int)(b > cap ? cap : b);
@@ -225,7 +231,7 @@ int permute_t(const void* x, int Tn, int H, const int32_t* row_slot, int k, cons
               cudaStream_t s) {
   using V = Vec<T, VB>;
   const int HV = H / V::n, tpt = threads_per_token(HV), tb = blocks_for(Tn, kPermThreads / tpt, 64);
-  CBMOE_CUDA_TRY(launch_pdl(permute_kernel<T, VB>, dim3(tb + pad_blocks(R, kPermThreads)), dim3(kPermThreads), 0, s,
+  CBMOE_CUDA_TRY(launch_pdl(permute_kernel<T, VB>, dim3(tb + pad_blocks(R, kPermThreads), row_blocks(HV, tpt, tb)), dim3(kPermThreads), 0, s,
                             static_cast<const V*>(x), Tn, HV, row_slot, k, tok_row, R, static_cast<V*>(xs), tb, tpt));
   return CBMOE_OK;
 }
@@ -235,9 +241,9 @@ int unpermute_t(const void* ys, int R, int H, const int32_t* row_slot, const flo
                 cudaStream_t s) {
   using V = Vec<T, VB>;
   const int HV = H / V::n;
-  const int tpt = threads_per_token(HV);
-  CBMOE_CUDA_TRY(launch_pdl(unpermute_kernel<T, VB>, dim3(blocks_for(Tn, kPermThreads / tpt, 64)), dim3(kPermThreads), 0,
-                            s, static_cast<const V*>(ys), R, HV, row_slot, w, Tn, k, static_cast<V*>(y), tpt));
+  const int tpt = threads_per_token(HV), tb = blocks_for(Tn, kPermThreads / tpt, 64);
+  CBMOE_CUDA_TRY(launch_pdl(unpermute_kernel<T, VB>, dim3(tb, row_blocks(HV, tpt, tb)), dim3(kPermThreads), 0, s,
+                            static_cast<const V*>(ys), R, HV, row_slot, w, Tn, k, static_cast<V*>(y), tpt));
   return CBMOE_OK;
 }
 

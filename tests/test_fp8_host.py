@@ -39,6 +39,9 @@ def test_linear_refusals(L):
                 dict(x=None), dict(y=None), dict(ldx=100), dict(x_type=4), dict(y_type=E4M3), dict(y_type=-1),
                 dict(x_type=E4M3), dict(x_type=E4M3, xs=16, ldx=136), dict(x_type=E4M3, xs=16, x=24)):
         assert linear(L, **bad) == INVALID, bad
+    assert linear(L, N=(1 << 30) + 1) == UNSUPPORTED
+    assert linear(L, K=(1 << 24) + 16, ldq=1 << 25, ldx=1 << 25) == UNSUPPORTED
+    assert linear(L, rows=0x7ffffe01) == INVALID
     assert linear(L, ws=None) == WORKSPACE
     assert linear(L, ws=264) == WORKSPACE                                         # not 256-byte aligned
     need = L.cbmoe_fp8_linear_workspace_bytes(1, 128, 4, BF16)

@@ -315,6 +315,58 @@ def test_experts_refusals():
         cbmoe.ResidentFetch(out_dtype=torch.float64).apply(p, x, idx, w, 0, 10.0)
 
 
+def test_experts_on_streams_and_in_graphs():
+    """Overlapping calls and two captured graphs share no scratch; a replay takes new values of the captured inputs."""
+    import cbmoe
+    rng = np.random.default_rng(16)
+    E, H, I, k = 6, 384, 256, 2
+    p, _ = layer(rng, E, H, I)
+    fetch = cbmoe.ResidentFetch(out_dtype=torch.bfloat16)
+    made = []
+    for N in (3, 50, 900):
+        idx, w = (torch.from_numpy(t).cuda() for t in gen.routing(rng, N, E, k))
+        made.append((activations(rng, N, H, torch.bfloat16), idx, w))
+    call = lambda c: fetch.apply(p, c[0], c[1], c[2], 0, gen.LIMIT)
+    want = [call(c) for c in made]
+    torch.cuda.synchronize()
+    got = []
+    for c in made:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got.append([call(c) for _ in range(3)])
+    torch.cuda.synchronize()
+    assert all(torch.equal(w, g) for w, gs in zip(want, got) for g in gs)
+    graphs = []
+    for c in made:
+        g = torch.cuda.CUDAGraph()
+        static = (c[0].clone(), c[1].clone(), c[2].clone())
+        with torch.cuda.graph(g):
+            y = call(static)
+        graphs.append((g, static, y))
+    for g, _, _ in graphs + graphs[::-1]:
+        g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(w, y) for w, (_, _, y) in zip(want, graphs))
+    g, static, y = graphs[1]
+    static[1].copy_(made[1][1].flip(0))
+    g.replay()
+    assert torch.equal(y, call((made[1][0], made[1][1].flip(0), made[1][2])))
+    no_device_errors()
+
+
+def test_many_tiles_with_a_cut_remainder():
+    """More tiles than pairs of SMs, the rest cut along K: whole and partial sums side by side, the same bits again."""
+    import cbmoe
+    rng = np.random.default_rng(17)
+    (q, s), (qn, sn) = table(rng, 128 * 21, 1500)
+    x = activations(rng, 2700, 1500, torch.float16)
+    y = cbmoe.ops.fp8_linear(q, s, x)
+    rows = rng.choice(2700, 64, replace=False)
+    want, bound = fp8.linear(qn, sn, f64(x)[rows], half_eps(torch.float32))
+    assert (np.abs(f64(y)[rows] - want) <= bound).all()
+    assert torch.equal(cbmoe.ops.fp8_linear(q, s, x), y)
+    no_device_errors()
+
+
 def test_router_plan_products_and_join_are_the_layer():
     """The operators one after another, as a program with its own expert loop uses them, against the fused layer."""
     import cbmoe
