@@ -53,7 +53,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__ x, int N, int K, long long ldx,
                                                            int vec, uint8_t* __restrict__ q, long long ldq,
                                                            float* __restrict__ s, int lds,
-                                                           const int* __restrict__ row_slot, int k, int R, int* __restrict__ zero, int n_zero) {
+                                                           const int* __restrict__ row_slot, int k, int R, int repeat, int* __restrict__ zero, int n_zero) {
   griddep_wait();
   griddep_launch();
   for (int i = blockIdx.x * 256 + threadIdx.x; i < n_zero; i += gridDim.x * 256) zero[i] = 0;
@@ -91,9 +91,9 @@ __global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__
     const uint2 o = make_uint2(fp8_pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
                                fp8_pack4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv));
     if (!in) continue;
-    const int copies = row_slot != nullptr ? k : 1;
+    const int copies = row_slot != nullptr ? k : repeat;
     for (int j = 0; j < copies; ++j) {
-      const int r = row_slot != nullptr ? row_slot[(size_t)n * k + j] : n;
+      const int r = row_slot != nullptr ? row_slot[(size_t)n * k + j] : n + 32 * j;
       if (r < 0 || r >= R) continue;
       uint8_t* dst = q + (size_t)r * ldq + c0;
       if (wide && c0 + 8 <= ldq) {
@@ -101,14 +101,17 @@ __global__ void __launch_bounds__(256) fp8_quantize_kernel(const T* __restrict__
       } else {
         for (int i = 0; i < 8 && c0 + i < K; ++i) dst[i] = (uint8_t)((i < 4 ? o.x : o.y) >> (8 * (i & 3)));
       }
-      if (l == 0) s[(size_t)r * lds + kb] = sc;
+      if (l == 0 && (row_slot != nullptr || j == 0)) s[(size_t)r * lds + kb] = sc;
     }
   }
 }
 
 // Scales that come with codes [N][KB] -> rows padded to whole 16-byte groups; clears the product's counters on the way.
+// Where q is given, also the codes [N][K], N <= 32, four times into q (rows n + 32 j of KB * 128 bytes).
 __global__ void __launch_bounds__(256) fp8_scales_kernel(const float* __restrict__ xs, int N, int KB, int ld,
-                                                         float* __restrict__ out, int* __restrict__ zero, int n_zero) {
+                                                         float* __restrict__ out, const uint8_t* __restrict__ x, int K,
+                                                         long long ldx, uint8_t* __restrict__ q, int* __restrict__ zero,
+                                                         int n_zero) {
   griddep_wait();
   griddep_launch();
   const long long total = (long long)N * ld, at = blockIdx.x * 256LL + threadIdx.x, step = gridDim.x * 256LL;
@@ -117,6 +120,24 @@ __global__ void __launch_bounds__(256) fp8_scales_kernel(const float* __restrict
     const long long n = i / ld;
     const int kb = (int)(i - n * ld);
     out[i] = kb < KB ? xs[n * KB + kb] : 0.f;
+  }
+  if (q == nullptr) return;
+  const int units = (K + 15) / 16;
+  for (long long i = at; i < (long long)N * units; i += step) {
+    const int n = (int)(i / units), c = (int)(i - (long long)n * units) * 16;
+    const uint8_t* src = x + n * ldx + c;
+    union {
+      uint4 v;
+      uint8_t b[16];
+    } u;
+    if (c + 16 <= K) {
+      u.v = *reinterpret_cast<const uint4*>(src);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) u.b[e] = c + e < K ? src[e] : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(q + (size_t)(n + 32 * j) * KB * kFp8Group + c) = u.v;
   }
 }
 
@@ -130,7 +151,10 @@ template <int MT, int TN>
 struct Fp8Cfg {
   static constexpr bool kPair = MT == 256;               // two CTAs, 128 tokens each
   static constexpr int kRows = kPair ? 128 : MT;         // tokens of a CTA's tile
-  static constexpr int kATile = kRows * 128;
+  // 32 tokens lie four times in the 128 rows of the M side: each TMEM lane quadrant holds all of them and its warps take a
+  // quarter of the columns. (Once, all columns would be read and summed by the two warps of one scheduler.)
+  static constexpr int kCopies = MT == 32 ? 4 : 1;
+  static constexpr int kATile = kCopies * kRows * 128;
   static constexpr int kBTile = (kPair ? TN / 2 : TN) * 128;
   // Column blocks per stage and per accumulator (256 columns in all): a hand-over costs some 500 clocks of the issuer and
   // of the promotion warps whatever its size, so narrow tiles take several blocks at once.
@@ -231,18 +255,19 @@ template <int W, typename OUT, int N>
 __device__ __forceinline__ void store_row(void* out, size_t row, int rows, int col0, const float (&acc)[N]) {
   const int end = min(rows - col0, W);
   OUT* dst = static_cast<OUT*>(out) + row * rows + col0;
-  constexpr int kU = 32 / (int)sizeof(OUT);
-  if (rows % kU == 0 && (reinterpret_cast<uintptr_t>(out) & 31) == 0) {
+  constexpr int kB = W * (int)sizeof(OUT) < 32 ? 16 : 32, kU = kB / (int)sizeof(OUT);
+  if (rows % kU == 0 && (reinterpret_cast<uintptr_t>(out) & (kB - 1)) == 0) {
 #pragma unroll
     for (int u = 0; u < W / kU; ++u) {
       if (u * kU < end) {
         union {
-          uint32_t w[8];
+          uint32_t w[kB / 4];
           OUT o[kU];
         } b;
 #pragma unroll
         for (int i = 0; i < kU; ++i) b.o[i] = out_of<OUT>(acc[u * kU + i]);
-        store32(dst + u * kU, b.w);
+        if constexpr (kB == 32) store32(dst + u * kU, b.w);
+        else *reinterpret_cast<uint4*>(dst + u * kU) = make_uint4(b.w[0], b.w[1], b.w[2], b.w[3]);
       }
     }
   } else {
@@ -293,7 +318,7 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const Fp8Param
       mbar_init(&d_full[i], 1);
       mbar_init(&d_empty[i], C::kPair ? 16 : 8);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(&meet[i], 2);
+    for (int i = 0; i < 4; ++i) mbar_init(&meet[i], C::kCopies > 1 ? 8 : 2);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -353,7 +378,9 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const Fp8Param
             weights(it, u, st);
 #pragma unroll
             for (int j = 0; j < C::kU; ++j)
-              tma_load_2d(smem + st * C::kStage + j * C::kATile, &map_x, (u * C::kU + j) * kFp8Group, xrow, &full[st]);
+              for (int i = 0; i < (p.g.repeated ? 1 : C::kCopies); ++i)
+                tma_load_2d(smem + st * C::kStage + j * C::kATile + i * C::kRows * 128, &map_x, (u * C::kU + j) * kFp8Group,
+                            xrow, &full[st]);
           }
           __syncwarp();
           if (++st == C::kNStage) {
@@ -426,7 +453,11 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const Fp8Param
     Fp8Sched sched = schedule();
     const int q = warp & 3;                  // TMEM lane quadrant this warp may read
     const int half = (warp - kW0) >> 2;
-    const int m = 32 * q + lane;             // this thread's row of the CTA's tile
+    const int qq = C::kCopies > 1 ? q : 0;   // quarter of the columns
+    const int m = C::kCopies > 1 ? lane : 32 * q + lane;   // this thread's row of the CTA's tile
+    constexpr int AC = TN / 2 / C::kCopies;  // columns of a warp (SwiGLU: half of gate, half of up)
+    constexpr int LW = AC < 16 ? AC : 16;    // columns of a load
+    uint64_t* const meet_bar = &meet[C::kCopies > 1 ? 0 : q];
     uint32_t n = 0, met = 0;
     auto d_read = [&](int buf) {             // to the CTA that issues the MMAs
       __syncwarp();
@@ -445,18 +476,18 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const Fp8Param
     bool have = sched.next(sg);
     if (have) it = item_of(sg);
     while (have) {
-      const bool live = 32 * q < it.cnt, mine = m < it.cnt;
+      const bool live = m - lane < it.cnt, mine = m < it.cnt;
       const size_t xrow = mine ? (size_t)it.row0 + m : 0;
       const bool have_n = sched.next(sn);
       if (have_n) itn = item_of(sn);         // under way while this tile is summed
-      float acc[TN / 2];
+      float acc[AC];
 #pragma unroll
-      for (int i = 0; i < TN / 2; ++i) acc[i] = 0.f;
+      for (int i = 0; i < AC; ++i) acc[i] = 0.f;
       // This row's scales, four blocks at a time (rows are padded to whole groups: fp8_scale_stride), and the weights', a
       // block per lane: of this half's 128-row block, or of gate and up. Fetched at least four blocks ahead of their use: a
       // load's latency under the tiles' traffic is longer than a block.
       const float* sx = p.g.xs + xrow * p.g.ldxs;
-      const int blk = SWIGLU ? it.nt : min((it.nt * TN + half * (TN / 2)) / 128, p.RB - 1), kb0 = sg.kb0 * C::kU;
+      const int blk = SWIGLU ? it.nt : min((it.nt * TN + half * (TN / 2) + AC * qq) / 128, p.RB - 1), kb0 = sg.kb0 * C::kU;
       const float* sa = p.g.s0 + ((size_t)it.e * p.RB + blk) * p.KB;
       const float* sb = SWIGLU ? p.g.s1 + ((size_t)it.e * p.RB + blk) * p.KB : sa;
       auto row_scales = [&](int kb) { return *reinterpret_cast<const float4*>(sx + min(kb, (p.KB - 1) & ~3)); };
@@ -497,18 +528,22 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const Fp8Param
           // 16 columns at a time: the two warps of a scheduler take turns between a load and its multiply-adds, and
           // 128 + 16 registers a thread leave nothing to spill (one spilled register in this loop costs more than any
           // longer load gains).
+          constexpr int kLoads = 128 / C::kCopies / LW;
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {         // SwiGLU: 0-3 gate, 4-7 up; else kU blocks of TN / 32
-            float v[16];
-            const int j = SWIGLU ? 0 : 16 * c / (TN / 2), at = SWIGLU ? 16 * c : 16 * c % (TN / 2);
-            tmem_ld16(t0 + (SWIGLU ? (c < 4 ? 0 : 64) + 64 * half + 16 * c : j * TN + TN / 2 * half + at), v);
-            if (c == 7) {                       // all of this unit is in registers
+          for (int c = 0; c < kLoads; ++c) {    // SwiGLU: gate, then up; else kU blocks
+            float v[LW];
+            const int j = SWIGLU ? 0 : LW * c / AC, at = LW * c % AC;
+            const int col = SWIGLU ? (at < AC / 2 ? 0 : 128) + 64 * half + AC / 2 * qq + at % (AC / 2)
+                                   : j * TN + TN / 2 * half + AC * qq + at;
+            if constexpr (LW == 16) tmem_ld16(t0 + col, v);
+            else tmem_ld8(t0 + col, v);
+            if (c == kLoads - 1) {              // all of this unit is in registers
               tc_fence_before();
               d_read(buf);
             }
-            const float f = SWIGLU && c >= 4 ? fb : fa[j];
+            const float f = SWIGLU && at >= AC / 2 ? fb : fa[j];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) acc[at + i] = fmaf(v[i], f, acc[at + i]);
+            for (int i = 0; i < LW; ++i) acc[at + i] = fmaf(v[i], f, acc[at + i]);
           }
         } else {
           d_read(buf);
@@ -516,26 +551,26 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const Fp8Param
       }
       bool whole = true;
       if (sg.kb1 - sg.kb0 < KBU) {
-        // ---------------- a range of the sum: partial sums [slot][rank][half][4-column group][row], 512 contiguous bytes a store
+        // ---------------- a range of the sum: partial sums [slot][rank][half][quarter][4-column group][row], 512 contiguous bytes a store
         int c0, c1;
         sched.sharers(sg.item, c0, c1);
         auto part = [&](int w) {
-          const size_t at = ((size_t)sched.slot(w, sg.item) * group + rank) * 2 + half;
-          return reinterpret_cast<float4*>(p.g.part) + at * (TN / 8) * C::kRows + m;
+          const size_t at = (((size_t)sched.slot(w, sg.item) * group + rank) * 2 + half) * C::kCopies + qq;
+          return reinterpret_cast<float4*>(p.g.part) + at * (AC / 4) * C::kRows + m;
         };
         if (mine) {
           float4* dst = part(sched.worker);
 #pragma unroll
-          for (int i = 0; i < TN / 8; ++i)
+          for (int i = 0; i < AC / 4; ++i)
             __stcg(dst + i * C::kRows, make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]));
         }
         __threadfence();
         int* arrived = p.g.arrived + ((sg.item - sched.first) * group + rank) * 8;
-        if constexpr (SWIGLU) {                            // one decision for the two halves of a row
-          if (!pair_meet(&meet[q], met)) goto late;        // both are written
-          const int at = (met & 1) * 4 + q;
-          if (half == 0 && lane == 0) flag[at] = atomicAdd(&arrived[q], 1) == c1 - c0;
-          if (!pair_meet(&meet[q], met)) goto late;
+        if constexpr (SWIGLU) {                            // one decision for all of a row
+          if (!pair_meet(meet_bar, met)) goto late;        // both are written
+          const int at = (met & 1) * 4 + (C::kCopies > 1 ? 0 : q);
+          if (half == 0 && lane == 0 && (C::kCopies == 1 || q == 0)) flag[at] = atomicAdd(&arrived[q], 1) == c1 - c0;
+          if (!pair_meet(meet_bar, met)) goto late;
           whole = flag[at] != 0;
         } else {
           int old = 0;
@@ -546,17 +581,18 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const Fp8Param
         if (whole) __threadfence();
         // The last worker to arrive adds the tile's ranges in their order, 8 loads under way at once.
 #pragma unroll
-        for (int i = 0; i < TN / 2; ++i) acc[i] = 0.f;
+        for (int i = 0; i < AC; ++i) acc[i] = 0.f;
         if (whole && mine) {
           for (int w = c0; w <= c1; ++w) {
             const float4* src = part(w);
+            constexpr int kStep = AC / 4 < 8 ? AC / 4 : 8;
 #pragma unroll
-            for (int i = 0; i < TN / 8; i += 8) {
-              float4 v[8];
+            for (int i = 0; i < AC / 4; i += kStep) {
+              float4 v[kStep];
 #pragma unroll
-              for (int j = 0; j < 8; ++j) v[j] = __ldcg(src + (i + j) * C::kRows);
+              for (int j = 0; j < kStep; ++j) v[j] = __ldcg(src + (i + j) * C::kRows);
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
+              for (int j = 0; j < kStep; ++j) {
                 acc[4 * (i + j)] += v[j].x;
                 acc[4 * (i + j) + 1] += v[j].y;
                 acc[4 * (i + j) + 2] += v[j].z;
@@ -571,23 +607,32 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const Fp8Param
       if (whole) {
         if constexpr (SWIGLU) {
           static_assert(!SWIGLU || TN == 256, "a row's maximum over 128 columns is taken inside one tile");
-          const int col0 = it.nt * 128 + 64 * half;
+          constexpr int GW = AC / 2;
+          const int col0 = it.nt * 128 + 64 * half + GW * qq;
           float top = 0.f;
 #pragma unroll
-          for (int i = 0; i < 64; ++i) {
-            acc[i] = col0 + i < rows ? swiglu_keep_nan(acc[i], acc[64 + i], p.g.limit) : 0.f;
+          for (int i = 0; i < GW; ++i) {
+            acc[i] = col0 + i < rows ? swiglu_keep_nan(acc[i], acc[GW + i], p.g.limit) : 0.f;
             top = max_nan(top, fabsf(acc[i]));
           }
-          float* mx = row_max + ((met & 1) * 4 + q) * 64;
-          mx[half * 32 + lane] = top;
-          if (!pair_meet(&meet[q], met)) goto late;
-          top = max_nan(top, mx[(half ^ 1) * 32 + lane]);
+          if constexpr (C::kCopies > 1) {
+            float* mx = row_max + (met & 1) * 256;
+            mx[(half * 4 + q) * 32 + lane] = top;
+            if (!pair_meet(meet_bar, met)) goto late;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = max_nan(top, mx[i * 32 + lane]);
+          } else {
+            float* mx = row_max + ((met & 1) * 4 + q) * 64;
+            mx[half * 32 + lane] = top;
+            if (!pair_meet(meet_bar, met)) goto late;
+            top = max_nan(top, mx[(half ^ 1) * 32 + lane]);
+          }
           float inv;
           const float sc = fp8_group_scale(top, &inv);
           if (mine) {
             uint4* dst = reinterpret_cast<uint4*>(p.g.hq + xrow * ((size_t)p.RB * 128) + col0);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
+            for (int u = 0; u < GW / 16; ++u) {
               uint32_t w[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
@@ -596,13 +641,13 @@ __global__ void __launch_bounds__(kFp8Threads, 1) fp8_gemm_kernel(const Fp8Param
               }
               dst[u] = make_uint4(w[0], w[1], w[2], w[3]);
             }
-            if (half == 0) p.g.hs[xrow * p.hs_ld + it.nt] = sc;
+            if (half == 0 && qq == 0) p.g.hs[xrow * p.hs_ld + it.nt] = sc;
           }
         } else if (mine) {
-          const int col0 = it.nt * TN + half * (TN / 2);
-          if (p.g.out_type == CBMOE_BF16) store_row<TN / 2, __nv_bfloat16>(p.g.out, xrow, rows, col0, acc);
-          else if (p.g.out_type == CBMOE_F16) store_row<TN / 2, __half>(p.g.out, xrow, rows, col0, acc);
-          else store_row<TN / 2, float>(p.g.out, xrow, rows, col0, acc);
+          const int col0 = it.nt * TN + half * (TN / 2) + AC * qq;
+          if (p.g.out_type == CBMOE_BF16) store_row<AC, __nv_bfloat16>(p.g.out, xrow, rows, col0, acc);
+          else if (p.g.out_type == CBMOE_F16) store_row<AC, __half>(p.g.out, xrow, rows, col0, acc);
+          else store_row<AC, float>(p.g.out, xrow, rows, col0, acc);
         }
       }
       sg = sn;
@@ -649,7 +694,7 @@ int launch_t(const Fp8Gemm& g, cudaStream_t stream) {
   p.NT = SWIGLU ? p.RB : (g.rows + TN - 1) / TN;
   p.hs_ld = fp8_scale_stride(g.rows);
   CUtensorMap mx, m0, m1;
-  int rc = make_fp8_map(&mx, g.xq, g.K, g.x_rows, g.ldx, C::kRows);
+  int rc = make_fp8_map(&mx, g.xq, g.K, g.repeated ? 128 : g.x_rows, g.ldx, g.repeated ? 128 : C::kRows);
   if (!rc) rc = make_fp8_map(&m0, g.w0, g.K, (long long)g.E * g.rows, g.ldw, TN / 2);
   if (!rc) rc = make_fp8_map(&m1, SWIGLU ? g.w1 : g.w0, g.K, (long long)g.E * g.rows, g.ldw, TN / 2);
   if (rc) return rc;
@@ -682,12 +727,14 @@ int launch_t(const Fp8Gemm& g, cudaStream_t stream) {
   return CBMOE_OK;
 }
 
-// Weight rows per tile with few tokens, by how many tiles that gives (for experts: at most one pass per slot is counted).
-// Measured on one B200: 5120 -> 12288, 1 token: 48 tiles of 256 25.8 us, 96 of 128 15.5, 192 of 64 19.2; 77 x 5000 -> 1411:
-// 6 of 256 26.8, 12 of 128 20.0, 23 of 64 16.3; the down product of 54 experts, 1080 tiles of 256: 119 us at either width.
+// Weight rows per tile with few tokens. Dense: by how many tiles that gives. Measured on one B200, quantiser included:
+// 5120 -> 12288, 64 tokens: 48 tiles of 256 28.9 us, 96 of 128 19.1, 192 of 64 22.8; 77 x 5000 -> 1411: 6 of 256 27.3, 12 of
+// 128 22.3, 23 of 64 18.7. Experts with up to 32 rows a pass load the tokens four times, so a block more per stage costs
+// four more loads: 256 (54 experts: 227 us against 242 at 128).
 template <int MT>
 int launch_few(const Fp8Gemm& g, cudaStream_t s) {
   if (g.w1 != nullptr) return launch_t<MT, 256, true>(g, s);
+  if (MT == 32 && g.pass_expert != nullptr) return launch_t<MT, 256, false>(g, s);
   const long long passes = g.pass_expert ? (g.x_rows < g.E ? g.x_rows : g.E) : (g.x_rows + MT - 1) / MT;
   if (passes * ((g.rows + 255) / 256) >= 2LL * num_sms()) return launch_t<MT, 256, false>(g, s);
   if (passes * ((g.rows + 127) / 128) >= num_sms() / 2) return launch_t<MT, 128, false>(g, s);
@@ -724,7 +771,7 @@ int launch_fp8_gemm(const Fp8Gemm& g, int mt, cudaStream_t s) {
 }
 
 int launch_fp8_quantize(const void* x, int type, int N, int K, long long ldx, uint8_t* q, long long ldq, float* s, int lds,
-                        const int* row_slot, int k, int R, int* zero, int n_zero, cudaStream_t stream) {
+                        const int* row_slot, int k, int R, int repeat, int* zero, int n_zero, cudaStream_t stream) {
   const long long groups = (long long)N * blocks_of(K);
   long long blocks = (groups + 15) / 16, cap = (long long)num_sms() * 16;
   if (blocks > cap) blocks = cap;
@@ -733,15 +780,15 @@ int launch_fp8_quantize(const void* x, int type, int N, int K, long long ldx, ui
   prof_begin(kProfOther, stream);
   if (type == CBMOE_BF16)
     CBMOE_CUDA_TRY(launch_pdl(fp8_quantize_kernel<__nv_bfloat16>, dim3((int)blocks), dim3(256), 0, stream,
-                              static_cast<const __nv_bfloat16*>(x), N, K, ldx, vec, q, ldq, s, lds, row_slot, k, R, zero,
+                              static_cast<const __nv_bfloat16*>(x), N, K, ldx, vec, q, ldq, s, lds, row_slot, k, R, repeat, zero,
                               n_zero));
   else if (type == CBMOE_F16)
     CBMOE_CUDA_TRY(launch_pdl(fp8_quantize_kernel<__half>, dim3((int)blocks), dim3(256), 0, stream,
-                              static_cast<const __half*>(x), N, K, ldx, vec, q, ldq, s, lds, row_slot, k, R, zero,
+                              static_cast<const __half*>(x), N, K, ldx, vec, q, ldq, s, lds, row_slot, k, R, repeat, zero,
                               n_zero));
   else
     CBMOE_CUDA_TRY(launch_pdl(fp8_quantize_kernel<float>, dim3((int)blocks), dim3(256), 0, stream,
-                              static_cast<const float*>(x), N, K, ldx, vec, q, ldq, s, lds, row_slot, k, R, zero,
+                              static_cast<const float*>(x), N, K, ldx, vec, q, ldq, s, lds, row_slot, k, R, repeat, zero,
                               n_zero));
   prof_end(kProfOther, stream);
   CBMOE_CUDA_TRY(cudaGetLastError());
@@ -750,7 +797,7 @@ int launch_fp8_quantize(const void* x, int type, int N, int K, long long ldx, ui
 
 namespace {
 
-// Workspace of a product: partial sums | counters | q [N][blocks * 128] (where x is quantised here) |
+// Workspace of a product: partial sums | counters | q [rows][blocks * 128] |
 // scales [N][fp8_scale_stride].
 struct LinearWs {
   size_t arrived, xq, xs, total;
@@ -761,7 +808,8 @@ LinearWs linear_ws(int N, int K, bool ready) {
   w.mt = fp8_pass_tokens(N, 1);
   w.arrived = lyr::align_up(fp8_part_bytes(w.mt));
   w.xq = w.arrived + lyr::align_up((size_t)fp8_arrived() * 4);
-  w.xs = w.xq + (ready ? 0 : lyr::align_up((size_t)N * blocks_of(K) * kFp8Group));
+  const int q_rows = w.mt == 32 ? 128 : (ready ? 0 : N);   // up to 32 tokens lie there four times
+  w.xs = w.xq + lyr::align_up((size_t)q_rows * blocks_of(K) * kFp8Group);
   w.total = w.xs + lyr::align_up((size_t)N * fp8_scale_stride(K) * 4);
   return w;
 }
@@ -812,7 +860,7 @@ extern "C" int cbmoe_fp8_quantize(const void* x, int type, int N, int K, long lo
   if (!type_ok(type) || N < 0 || K <= 0 || ldx < K || ldq < K) return CBMOE_ERR_INVALID;
   if (N == 0) return CBMOE_OK;
   if (!x || !q || !s) return CBMOE_ERR_INVALID;
-  return launch_fp8_quantize(x, type, N, K, ldx, q, ldq, s, blocks_of(K), nullptr, 1, N, nullptr, 0, stream);
+  return launch_fp8_quantize(x, type, N, K, ldx, q, ldq, s, blocks_of(K), nullptr, 1, N, 1, nullptr, 0, stream);
 }
 
 extern "C" size_t cbmoe_fp8_linear_workspace_bytes(int N, int K, int rows, int x_type) {
@@ -850,17 +898,25 @@ extern "C" int cbmoe_fp8_linear(const void* q, long long ldq, const float* s, in
     g.ldx = ldx;
     g.xs = sc;
     g.ldxs = fp8_scale_stride(K);
-    const long long blocks = ((long long)N * g.ldxs + 255) / 256, cap = num_sms() * 8;
+    if (W.mt == 32) {
+      g.xq = ws + W.xq;
+      g.ldx = (long long)blocks_of(K) * kFp8Group;
+      g.repeated = 1;
+    }
+    const long long blocks = ((long long)N * (W.mt == 32 ? K / 16 + g.ldxs : g.ldxs) + 255) / 256, cap = num_sms() * 8;
     prof_begin(kProfOther, stream);
     CBMOE_CUDA_TRY(launch_pdl(fp8_scales_kernel, dim3((int)(blocks < cap ? blocks : cap)), dim3(256), 0, stream, xs, N,
-                              blocks_of(K), g.ldxs, sc, g.arrived, fp8_arrived()));
+                              blocks_of(K), g.ldxs, sc, static_cast<const uint8_t*>(x), K, ldx,
+                              W.mt == 32 ? ws + W.xq : static_cast<uint8_t*>(nullptr), g.arrived, fp8_arrived()));
     prof_end(kProfOther, stream);
     CBMOE_CUDA_TRY(cudaGetLastError());
   } else {
     float* sc = reinterpret_cast<float*>(ws + W.xs);
     g.ldxs = fp8_scale_stride(K);
     g.ldx = (long long)blocks_of(K) * kFp8Group;
-    const int rc = launch_fp8_quantize(x, x_type, N, K, ldx, ws + W.xq, g.ldx, sc, g.ldxs, nullptr, 1, N, g.arrived,
+    g.repeated = W.mt == 32;
+    const int rc = launch_fp8_quantize(x, x_type, N, K, ldx, ws + W.xq, g.ldx, sc, g.ldxs, nullptr, 1,
+                                       g.repeated ? 128 : N, g.repeated ? 4 : 1, g.arrived,
                                        fp8_arrived(), stream);
     if (rc) return rc;
     g.xq = ws + W.xq;
@@ -899,7 +955,7 @@ extern "C" int cbmoe_fp8_experts_apply(const cbmoe_fp8_experts* ex, const uint16
   g.xq = ws + W.xq;
   g.xs = reinterpret_cast<const float*>(ws + W.xs);
   rc = launch_fp8_quantize(x, CBMOE_BF16, N, ex->H, ex->H, ws + W.xq, g.ldx, reinterpret_cast<float*>(ws + W.xs), g.ldxs,
-                           row_slot, k, W.Rp, arrived, 2 * fp8_arrived(), stream);
+                           row_slot, k, W.Rp, 1, arrived, 2 * fp8_arrived(), stream);
   if (rc) return rc;
   g.part = reinterpret_cast<float*>(ws + W.part);
   g.arrived = arrived;

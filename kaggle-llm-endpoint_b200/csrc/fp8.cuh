@@ -45,6 +45,7 @@ struct Fp8Gemm {
   const void* xq;          // e4m3 [x_rows][ldx]
   long long ldx;
   int x_rows;
+  int repeated;            // dense, up to 32 tokens: xq holds row n at n, 32 + n, 64 + n and 96 + n
   const float* xs;         // [x_rows][ldxs], ldxs = fp8_scale_stride(K), 16-byte aligned
   int ldxs;
   const void* w0;          // e4m3 [E][rows][ldw]; w1: up, beside w0 = gate (SwiGLU), else null
@@ -76,8 +77,9 @@ int fp8_arrived();         // counters of one launch: 8 for each tile that can b
 int launch_fp8_gemm(const Fp8Gemm& g, int mt, cudaStream_t s);
 // x [N][K] (row stride ldx elements) -> e4m3 rows q (stride ldq bytes, columns K.. up to ldq zero where a unit of 8
 // reaches past K) and scales s [..][lds]; with row_slot, row n goes to the k rows row_slot[n][:] in [0, R).
+// With `repeat` (row_slot null) row n goes to the rows n + 32 j, j < repeat, its scales to row n only.
 // Clears zero[0, n_zero) on the way (the counters of the products that follow).
 int launch_fp8_quantize(const void* x, int type, int N, int K, long long ldx, uint8_t* q, long long ldq, float* s, int lds,
-                        const int* row_slot, int k, int R, int* zero, int n_zero, cudaStream_t stream);
+                        const int* row_slot, int k, int R, int repeat, int* zero, int n_zero, cudaStream_t stream);
 
 }  // namespace cbmoe
