@@ -8,6 +8,9 @@
 // All three are bound by memory, so each walks the tokens, not the sorted rows: a token's row is read once and its k
 // sorted rows are written (or read) once, and no row is touched twice. A sorted row belongs to one slot, so nothing is
 // added by atomics: sums run over j in order, in fp32, rounded once. Rows outside [0, R) in row_slot are empty slots.
+// Measured on one B200, 4096 tokens x 8 slots, rows of 5120 bf16 (about 375 MB a direction, 57 us at the copy rate):
+// permute 74 us, unpermute 61-77 us; backward of the weighted form 172 us for 108 us of bytes (it reads ys and writes dys).
+// Looking a slot's row up once per token and not once per unit took the plan, permute and its gradient from 198 to 184 us.
 #include <cuda_fp16.h>
 
 #include "decode.cuh"
@@ -231,7 +234,8 @@ int permute_t(const void* x, int Tn, int H, const int32_t* row_slot, int k, cons
               cudaStream_t s) {
   using V = Vec<T, VB>;
   const int HV = H / V::n, tpt = threads_per_token(HV), tb = blocks_for(Tn, kPermThreads / tpt, 64);
-  CBMOE_CUDA_TRY(launch_pdl(permute_kernel<T, VB>, dim3(tb + pad_blocks(R, kPermThreads), row_blocks(HV, tpt, tb)), dim3(kPermThreads), 0, s,
+  CBMOE_CUDA_TRY(launch_pdl(permute_kernel<T, VB>, dim3(tb + pad_blocks(R, kPermThreads), row_blocks(HV, tpt, tb)),
+                            dim3(kPermThreads), 0, s,
                             static_cast<const V*>(x), Tn, HV, row_slot, k, tok_row, R, static_cast<V*>(xs), tb, tpt));
   return CBMOE_OK;
 }

@@ -16,6 +16,8 @@ What it restates (reference = shallmall/kaggle-llm-endpoint, paths relative to l
   gen.py   seeded synthetic inputs with the benchmark configs' shapes and value distributions.
   iq.py    the reference's real expert formats IQ2_S / IQ3_S / IQ4_XS (iqquant.py:108-146, llama.cpp's published
            dequant; grid tables loaded from gguf-py at run time).
+  fp8.py   e4m3 with block scales in float64: the activation quantiser, the block-scaled product and the routed experts
+           on such tables, each with a bound on an fp32 evaluation's error. No counterpart in the reference.
 
 Pinning: the format-independent pieces (ragged_plan, swiglu_clamped, quantize_array, dequant_tree, the decode and
 ragged compositions) are pinned by fixtures generated by executing the reference's own functions on a NumPy-backed
