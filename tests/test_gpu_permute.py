@@ -87,6 +87,45 @@ def test_unpermute_and_gradients(T, E, k, H, tm, dtype, empty):
     assert torch.equal(again[0], dys) and torch.equal(again[1], dw)        # the same bits again
 
 
+@pytest.mark.parametrize("H", [20, 132, 1282, 2564])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shift", [0, 1, 2, 4])
+def test_units_of_a_row(H, dtype, shift):
+    """Rows and pointers aligned to 2, 4, 8 and 16 bytes (views `shift` elements into their storage): the same values
+    whatever the width of a load, and nothing written outside."""
+    import cbmoe
+    T, E, k, tm = 37, 6, 4, 8
+    plan, idx, w, new = case(T, E, k, H, tm, dtype, True)
+    slot, R = rows_of(plan, T, k, E, tm)
+
+    def moved(t):
+        flat = torch.empty(t.numel() + shift, dtype=t.dtype, device="cuda")
+        flat[shift:] = t.flatten()
+        return flat[shift:].view(t.shape)
+
+    x, ys, dy = new(T, H), new(R, H), new(T, H)
+    xs = cbmoe.moe_permute(moved(x), plan)
+    want = torch.zeros(R, H, dtype=x.dtype)
+    for j in range(k):
+        t = torch.nonzero(slot[:, j] >= 0)[:, 0]
+        want[slot[t, j]] = x.cpu()[t]
+    assert torch.equal(xs.cpu(), want)
+    a, wl = moved(ys).requires_grad_(), w.clone().requires_grad_()
+    y = cbmoe.moe_unpermute(a, wl, plan)
+    real = slot >= 0
+    rows = torch.where(real[..., None], ys.double().cpu()[slot.clamp_min(0)], 0.0)
+    terms = w.double().cpu()[..., None] * rows
+    he = torch.finfo(ys.dtype).eps / 2
+    bound = k * 2.0 ** -24 * terms.abs().sum(1) * 1.001
+    assert ((y.detach().double().cpu() - terms.sum(1)).abs() <= bound + he * (terms.sum(1).abs() + bound) + 2.0 ** -25).all()
+    dys, dw = torch.autograd.grad(y, (a, wl), moved(dy))
+    want = torch.zeros(R, H, dtype=torch.float64)
+    want[slot[real]] = (w.double().cpu()[..., None] * dy.double().cpu()[:, None])[real]
+    assert ((dys.double().cpu() - want).abs() <= (he + 2.0 ** -24) * 1.001 * want.abs() + 2.0 ** -25).all()
+    prod = rows * dy.double().cpu()[:, None]
+    assert ((dw.double().cpu() - prod.sum(-1)).abs() <= (H / 128 + 18) * 2.0 ** -24 * prod.abs().sum(-1)).all()
+
+
 def test_gradients_against_differences():
     """Both operators are linear in each argument, so a central difference along a direction is exact up to rounding."""
     import cbmoe
