@@ -9,7 +9,7 @@
 // sorted rows are written (or read) once, and no row is touched twice. A sorted row belongs to one slot, so nothing is
 // added by atomics: sums run over j in order, in fp32, rounded once. Rows outside [0, R) in row_slot are empty slots.
 // Measured on one B200, 4096 tokens x 8 slots, rows of 5120 bf16 (about 375 MB a direction, 57 us at the copy rate):
-// permute 74 us, unpermute 61-77 us; backward of the weighted form 172 us for 108 us of bytes (it reads ys and writes dys).
+// permute 67 us, unpermute 70-78 us; backward of the weighted form 150 us for 108 us of bytes (it reads ys and writes dys).
 // Looking a slot's row up once per token and not once per unit took the plan, permute and its gradient from 198 to 184 us.
 #include <cuda_fp16.h>
 
@@ -41,7 +41,7 @@ struct Elem<float> {
 };
 
 // VB bytes of a row as one unit: the most of 16, 8, 4 and 2 that rows and pointers are aligned to.
-// 4096 x 8 rows of 2564 bf16 (8 bytes): permute 42 us, unpermute 61, backward 90; by single elements 76, 117 and 151.
+// 4096 x 8 rows of 2564 bf16 (8 bytes): permute 41 us, unpermute 56, backward 90; by single elements 76, 117 and 151.
 template <typename T, int VB>
 struct alignas(VB) Vec {
   static constexpr int n = VB / (int)sizeof(T);
@@ -110,30 +110,66 @@ __global__ void __launch_bounds__(kPermThreads) unpermute_kernel(const Vec<T, VB
   griddep_launch();
   const int per = kPermThreads / tpt, c0 = threadIdx.x % tpt + tpt * blockIdx.y, dc = tpt * gridDim.y;
   for (int t = blockIdx.x * per + threadIdx.x / tpt; t < Tn; t += gridDim.x * per) {
-    for (int c = c0; c < HV; c += dc) {
-      float acc[V::n] = {};
-      for (int j0 = 0; j0 < k; j0 += 8) {   // 8 rows in flight
-        V v[8];
-        float wt[8];
-        bool in[8];
+    // Units under 16 bytes are many, so their rows are looked up once per token (8 slots at most): 61 -> 56 us for 4096 x 8
+    // rows of 2564 bf16, 84 -> 64 for 2562. With whole units the registers that it holds cost more: 42 -> 49 for 2560.
+    if constexpr (VB < 16) {
+      int r[8];
+      float wt[8];
+      const auto look_up = [&](int j0) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int r = j0 + j < k ? row_slot[(size_t)t * k + j0 + j] : -1;
-          in[j] = r >= 0 && r < R;
-          wt[j] = in[j] && w != nullptr ? w[(size_t)t * k + j0 + j] : 1.f;
-          if (in[j]) v[j] = ys[(size_t)r * HV + c];
+          r[j] = j0 + j < k ? row_slot[(size_t)t * k + j0 + j] : -1;
+          if (r[j] >= R) r[j] = -1;
+          wt[j] = r[j] >= 0 && w != nullptr ? w[(size_t)t * k + j0 + j] : 1.f;
         }
+      };
+      look_up(0);
+      for (int c = c0; c < HV; c += dc) {
+        float acc[V::n] = {};
+        for (int j0 = 0; j0 < k; j0 += 8) {
+          V v[8];
+          if (k > 8) look_up(j0);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (in[j]) {
+          for (int j = 0; j < 8; ++j)
+            if (r[j] >= 0) v[j] = ys[(size_t)r[j] * HV + c];
 #pragma unroll
-            for (int q = 0; q < V::n; ++q) acc[q] = fmaf(wt[j], Elem<T>::to(v[j].v[q]), acc[q]);
-          }
+          for (int j = 0; j < 8; ++j)
+            if (r[j] >= 0) {
+#pragma unroll
+              for (int q = 0; q < V::n; ++q) acc[q] = fmaf(wt[j], Elem<T>::to(v[j].v[q]), acc[q]);
+            }
+        }
+        V o;
+#pragma unroll
+        for (int q = 0; q < V::n; ++q) o.v[q] = Elem<T>::from(acc[q]);
+        y[(size_t)t * HV + c] = o;
       }
-      V o;
+    } else {
+      for (int c = c0; c < HV; c += dc) {
+        float acc[V::n] = {};
+        for (int j0 = 0; j0 < k; j0 += 8) {   // 8 rows in flight
+          V v[8];
+          float wt[8];
+          bool in[8];
 #pragma unroll
-      for (int q = 0; q < V::n; ++q) o.v[q] = Elem<T>::from(acc[q]);
-      y[(size_t)t * HV + c] = o;
+          for (int j = 0; j < 8; ++j) {
+            const int r = j0 + j < k ? row_slot[(size_t)t * k + j0 + j] : -1;
+            in[j] = r >= 0 && r < R;
+            wt[j] = in[j] && w != nullptr ? w[(size_t)t * k + j0 + j] : 1.f;
+            if (in[j]) v[j] = ys[(size_t)r * HV + c];
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (in[j]) {
+#pragma unroll
+              for (int q = 0; q < V::n; ++q) acc[q] = fmaf(wt[j], Elem<T>::to(v[j].v[q]), acc[q]);
+            }
+        }
+        V o;
+#pragma unroll
+        for (int q = 0; q < V::n; ++q) o.v[q] = Elem<T>::from(acc[q]);
+        y[(size_t)t * HV + c] = o;
+      }
     }
   }
 }
@@ -223,6 +259,9 @@ int pad_blocks(int R, int threads) {
   return (int)(b > cap ? cap : b);
 }
 
+// The backward of 16-bit rows moves 8 bytes a thread at most: 8 rows of ys in whole units hold 32 registers more and leave
+// fewer warps. 4096 x 8 rows of 5120 bf16: 150 us against 172; of 2560: 82 against 105.
+int back_unit(int type, int unit) { return type != CBMOE_F32 && unit == 16 ? 8 : unit; }
 size_t elem_size(int type) { return type == CBMOE_F32 ? 4 : 2; }
 
 int unit_bytes(int type, int H, const void* a, const void* b, const void* c = nullptr) {
@@ -316,8 +355,9 @@ extern "C" int cbmoe_unpermute_backward(const void* dy, const void* ys, int type
   if (!dys && !dw) return CBMOE_OK;
   if (T == 0 && (!dys || R == 0)) return CBMOE_OK;
   prof_begin(kProfCombine, stream);
-  const int rc = CBMOE_BY_TYPE(unpermute_backward_t, type, unit_bytes(type, H, dy, dys, ys), dy, ys, R, H, row_slot,
-                               tok_row, w, T, k, dys, dw, stream);
+  const int unit = back_unit(type, unit_bytes(type, H, dy, dys, ys));
+  const int rc = CBMOE_BY_TYPE(unpermute_backward_t, type, unit, dy, ys, R, H, row_slot, tok_row, w, T, k, dys, dw,
+                               stream);
   prof_end(kProfCombine, stream);
   if (rc) return rc;
   CBMOE_CUDA_TRY(cudaGetLastError());
