@@ -9,7 +9,7 @@
 // sorted rows are written (or read) once, and no row is touched twice. A sorted row belongs to one slot, so nothing is
 // added by atomics: sums run over j in order, in fp32, rounded once. Rows outside [0, R) in row_slot are empty slots.
 // Measured on one B200, 4096 tokens x 8 slots, rows of 5120 bf16 (about 375 MB a direction, 57 us at the copy rate):
-// permute 67 us, unpermute 70-78 us; backward of the weighted form 150 us for 108 us of bytes (it reads ys and writes dys).
+// permute 67 us, unpermute 70 us; backward of the weighted form 150 us for 108 us of bytes (it reads ys and writes dys).
 // Looking a slot's row up once per token and not once per unit took the plan, permute and its gradient from 198 to 184 us.
 #include <cuda_fp16.h>
 
