@@ -255,7 +255,7 @@ int cbmoe_fp8_linear(const void* q, long long ldq, const float* s, int rows, int
  * [E][I][ld_in], down [E][H][ld_down] with scales [E][ceil(I/128)][ceil(H/128)] and [E][ceil(H/128)][ceil(I/128)].
  * x bf16 [N][H], idx int32 [N][k] (negative: empty slot), w fp32 [N][k] -> y [N][H] of y_type =
  * sum_j w[n, j] down_e(swiglu_clamped(gate_e x_n, up_e x_n, limit)); x and the SwiGLU output are quantised as above.
- * Each slot's output is rounded to y_type before the weighted fp32 sum. E <= 1024, k <= 64. */
+ * Each slot's output and the weighted sum are fp32, rounded once to y_type. E <= 1024, k <= 64. */
 typedef struct {
   int E, H, I;
   const void* gate;

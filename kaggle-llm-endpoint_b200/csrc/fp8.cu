@@ -820,12 +820,15 @@ LinearWs linear_ws(int N, int K, bool ready) {
 }
 
 // Workspace of the layer: plan | partial sums | counters (gate/up, down) | xq, xs (sorted rows) | hq, hs | slot outputs.
+// The slots' outputs are fp32 whatever the type of y: the weighted sum is rounded once, and a slot may lie outside the
+// range of fp16 where the sum does not. (160 experts x 4096 tokens, bf16 out: 1877 us a call; with slots in bf16, a second
+// rounding, 1728.)
 struct ExpertsWs {
   size_t plan, part, arrived, xq, xs, hq, hs, y, total;
   int mt, Rp;
   lyr::PlanLayoutHost L;
 };
-ExpertsWs experts_ws(int E, int H, int I, int N, int k, int y_type) {
+ExpertsWs experts_ws(int E, int H, int I, int N, int k) {
   ExpertsWs w;
   const long long S = (long long)N * k;
   w.mt = fp8_pass_tokens(S, E);
@@ -839,7 +842,7 @@ ExpertsWs experts_ws(int E, int H, int I, int N, int k, int y_type) {
   w.hq = w.xs + lyr::align_up((size_t)S * fp8_scale_stride(H) * 4);
   w.hs = w.hq + lyr::align_up((size_t)S * blocks_of(I) * kFp8Group);
   w.y = w.hs + lyr::align_up((size_t)S * fp8_scale_stride(I) * 4);
-  w.total = w.y + lyr::align_up((size_t)S * H * (y_type == CBMOE_F32 ? 4 : 2));
+  w.total = w.y + lyr::align_up((size_t)S * H * 4);
   return w;
 }
 
@@ -933,7 +936,7 @@ extern "C" int cbmoe_fp8_linear(const void* q, long long ldq, const float* s, in
 
 extern "C" size_t cbmoe_fp8_experts_workspace_bytes(const cbmoe_fp8_experts* ex, int N, int k, int y_type) {
   if (!ex || ex->E <= 0 || ex->H <= 0 || ex->I <= 0 || N < 0 || k <= 0 || !type_ok(y_type)) return 0;
-  return experts_ws(ex->E, ex->H, ex->I, N, k, y_type).total;
+  return experts_ws(ex->E, ex->H, ex->I, N, k).total;
 }
 
 extern "C" int cbmoe_fp8_experts_apply(const cbmoe_fp8_experts* ex, const uint16_t* x, int N, const int32_t* idx,
@@ -943,7 +946,7 @@ extern "C" int cbmoe_fp8_experts_apply(const cbmoe_fp8_experts* ex, const uint16
   if (N == 0) return CBMOE_OK;
   if (!x || !idx || !w || !y) return CBMOE_ERR_INVALID;
   if ((long long)N * k > (1 << 30)) return CBMOE_ERR_UNSUPPORTED;
-  const ExpertsWs W = experts_ws(ex->E, ex->H, ex->I, N, k, y_type);
+  const ExpertsWs W = experts_ws(ex->E, ex->H, ex->I, N, k);
   if (!workspace || workspace_bytes < W.total || !aligned(workspace, 256)) return CBMOE_ERR_WORKSPACE;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   int32_t* plan = reinterpret_cast<int32_t*>(ws + W.plan);
@@ -995,8 +998,9 @@ extern "C" int cbmoe_fp8_experts_apply(const cbmoe_fp8_experts* ex, const uint16
   d.hq = nullptr;
   d.hs = nullptr;
   d.out = ws + W.y;
-  d.out_type = y_type;
+  d.out_type = CBMOE_F32;
   rc = launch_fp8_gemm(d, W.mt, stream);
   if (rc) return rc;
-  return cbmoe_unpermute(ws + W.y, y_type, W.Rp, ex->H, row_slot, w, N, k, y, stream);
+  return launch_unpermute_f32(reinterpret_cast<const float*>(ws + W.y), W.Rp, ex->H, row_slot, w, N, k, y, y_type,
+                              stream);
 }

@@ -76,6 +76,10 @@ int routed_grouped(const cbmoe_experts* ex, const uint16_t* x, int N, const int3
 
 }  // namespace lyr
 
+// y[t] = sum_j w[t][j] * ys[row_slot[t][j]] of fp32 rows, rounded once to y_type (permute.cu; any H).
+int launch_unpermute_f32(const float* ys, int R, int H, const int32_t* row_slot, const float* w, int T, int k, void* y,
+                         int y_type, cudaStream_t stream);
+
 // Peer-memory transport of the expert-parallel layer (ep_peer.cu).
 struct EpPeer;
 bool ep_peer_matches(const EpPeer* pe, int nranks, int rank, int H, int cap);

@@ -14,6 +14,7 @@
 #include <cuda_fp16.h>
 
 #include "decode.cuh"
+#include "layer.cuh"
 #include "profile.cuh"
 
 namespace cbmoe {
@@ -47,6 +48,10 @@ struct alignas(VB) Vec {
   static constexpr int n = VB / (int)sizeof(T);
   T v[n];
 };
+
+// The sums of a unit of T as O.
+template <typename T, int VB, typename O>
+using Out = Vec<O, Vec<T, VB>::n * (int)sizeof(O)>;
 
 // Zero rows of `out` where tok_row < 0: a warp looks at up to 32 rows at a time, at fewer where there are enough warps
 // (a row of padding is a warp's work: 528 rows of 1411 halfs by 17 warps took 15 us).
@@ -100,11 +105,12 @@ __global__ void __launch_bounds__(kPermThreads) permute_kernel(const Vec<T, VB>*
   }
 }
 
-template <typename T, int VB>
+// Rows of T, sums rounded to O.
+template <typename T, int VB, typename O>
 __global__ void __launch_bounds__(kPermThreads) unpermute_kernel(const Vec<T, VB>* __restrict__ ys, int R, int HV,
                                                                  const int32_t* __restrict__ row_slot,
                                                                  const float* __restrict__ w, int Tn, int k,
-                                                                 Vec<T, VB>* __restrict__ y, int tpt) {
+                                                                 Out<T, VB, O>* __restrict__ y, int tpt) {
   using V = Vec<T, VB>;
   griddep_wait();
   griddep_launch();
@@ -139,9 +145,9 @@ __global__ void __launch_bounds__(kPermThreads) unpermute_kernel(const Vec<T, VB
               for (int q = 0; q < V::n; ++q) acc[q] = fmaf(wt[j], Elem<T>::to(v[j].v[q]), acc[q]);
             }
         }
-        V o;
+        Out<T, VB, O> o;
 #pragma unroll
-        for (int q = 0; q < V::n; ++q) o.v[q] = Elem<T>::from(acc[q]);
+        for (int q = 0; q < V::n; ++q) o.v[q] = Elem<O>::from(acc[q]);
         y[(size_t)t * HV + c] = o;
       }
     } else {
@@ -165,9 +171,9 @@ __global__ void __launch_bounds__(kPermThreads) unpermute_kernel(const Vec<T, VB
               for (int q = 0; q < V::n; ++q) acc[q] = fmaf(wt[j], Elem<T>::to(v[j].v[q]), acc[q]);
             }
         }
-        V o;
+        Out<T, VB, O> o;
 #pragma unroll
-        for (int q = 0; q < V::n; ++q) o.v[q] = Elem<T>::from(acc[q]);
+        for (int q = 0; q < V::n; ++q) o.v[q] = Elem<O>::from(acc[q]);
         y[(size_t)t * HV + c] = o;
       }
     }
@@ -281,14 +287,14 @@ int permute_t(const void* x, int Tn, int H, const int32_t* row_slot, int k, cons
   return CBMOE_OK;
 }
 
-template <typename T, int VB>
+template <typename T, int VB, typename O = T>
 int unpermute_t(const void* ys, int R, int H, const int32_t* row_slot, const float* w, int Tn, int k, void* y,
                 cudaStream_t s) {
   using V = Vec<T, VB>;
   const int HV = H / V::n;
   const int tpt = threads_per_token(HV), tb = blocks_for(Tn, kPermThreads / tpt, 64);
-  CBMOE_CUDA_TRY(launch_pdl(unpermute_kernel<T, VB>, dim3(tb, row_blocks(HV, tpt, tb)), dim3(kPermThreads), 0, s,
-                            static_cast<const V*>(ys), R, HV, row_slot, w, Tn, k, static_cast<V*>(y), tpt));
+  CBMOE_CUDA_TRY(launch_pdl(unpermute_kernel<T, VB, O>, dim3(tb, row_blocks(HV, tpt, tb)), dim3(kPermThreads), 0, s,
+                            static_cast<const V*>(ys), R, HV, row_slot, w, Tn, k, static_cast<Out<T, VB, O>*>(y), tpt));
   return CBMOE_OK;
 }
 
@@ -316,6 +322,37 @@ bool type_ok(int t) { return t == CBMOE_BF16 || t == CBMOE_F16 || t == CBMOE_F32
    : (type) == CBMOE_BF16 ? ((unit) == 2 ? f<__nv_bfloat16, 2>(__VA_ARGS__)                   \
                                          : CBMOE_BY_UNIT(f, __nv_bfloat16, unit, __VA_ARGS__)) \
                           : ((unit) == 2 ? f<__half, 2>(__VA_ARGS__) : CBMOE_BY_UNIT(f, __half, unit, __VA_ARGS__)))
+
+namespace {
+
+template <typename T, int VB>
+int unpermute_to_bf16(const void* ys, int R, int H, const int32_t* row_slot, const float* w, int Tn, int k, void* y,
+                      cudaStream_t s) {
+  return unpermute_t<T, VB, __nv_bfloat16>(ys, R, H, row_slot, w, Tn, k, y, s);
+}
+template <typename T, int VB>
+int unpermute_to_f16(const void* ys, int R, int H, const int32_t* row_slot, const float* w, int Tn, int k, void* y,
+                     cudaStream_t s) {
+  return unpermute_t<T, VB, __half>(ys, R, H, row_slot, w, Tn, k, y, s);
+}
+
+}  // namespace
+
+int launch_unpermute_f32(const float* ys, int R, int H, const int32_t* row_slot, const float* w, int T, int k, void* y,
+                         int y_type, cudaStream_t stream) {
+  // 16-bit rows of y are half as wide as those of ys: a unit of y is aligned where twice its address is
+  const uintptr_t y_as = reinterpret_cast<uintptr_t>(y) * (y_type == CBMOE_F32 ? 1 : 2);
+  const int unit = unit_bytes(CBMOE_F32, H, ys, reinterpret_cast<const void*>(y_as));
+  prof_begin(kProfCombine, stream);
+  const int rc = y_type == CBMOE_F32 ? CBMOE_BY_UNIT(unpermute_t, float, unit, ys, R, H, row_slot, w, T, k, y, stream)
+                 : y_type == CBMOE_BF16
+                     ? CBMOE_BY_UNIT(unpermute_to_bf16, float, unit, ys, R, H, row_slot, w, T, k, y, stream)
+                     : CBMOE_BY_UNIT(unpermute_to_f16, float, unit, ys, R, H, row_slot, w, T, k, y, stream);
+  prof_end(kProfCombine, stream);
+  if (rc) return rc;
+  CBMOE_CUDA_TRY(cudaGetLastError());
+  return CBMOE_OK;
+}
 
 }  // namespace cbmoe
 

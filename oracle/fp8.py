@@ -93,7 +93,6 @@ def experts(gate, up, down, x, idx, w, limit, half_eps):
                 step = np.maximum(step, np.abs(codes(v, sc) * spread(sc, h.shape[1]) - np.abs(hq)))
         o = hq @ wd.T
         eo = step @ np.abs(wd).T + sum_bound(h.shape[1]) * ((np.abs(hq) + step) @ np.abs(wd).T)
-        eo += half_eps * (np.abs(o) + eo)                # the slot's own rounding
         np.add.at(y, t, w[t, j][:, None] * o)
         np.add.at(bound, t, np.abs(w[t, j])[:, None] * eo)
         np.add.at(mag, t, np.abs(w[t, j])[:, None] * np.abs(o))

@@ -396,3 +396,37 @@ def test_router_plan_products_and_join_are_the_layer():
     # (2^-4 of that value). Per element of y: one of I = 256 terms; 2^-4 sqrt(1 / 256) of the norm is 2^-8.
     assert (y - fused).norm() <= 2.0 ** -8 * fused.norm()
     no_device_errors()
+
+
+@pytest.mark.parametrize("N,E,H,I,k", EXPERTS + [(9, 3, 131, 140, 3), (40, 16, 260, 128, 8)])
+@pytest.mark.parametrize("out", ["bf16", "fp16"])
+def test_experts_round_once(N, E, H, I, k, out):
+    """The slots' outputs stay in fp32 whatever the type of the result: 16 bits are the fp32 result rounded, no more."""
+    rng = np.random.default_rng(N + E + H + I + 1)
+    p, _ = layer(rng, E, H, I)
+    x = activations(rng, N, H, torch.bfloat16)
+    idx, w = gen.routing(rng, N, E, k)
+    y = apply(p, x, idx, w, TYPES[out])
+    assert torch.equal(y, apply(p, x, idx, w, torch.float32).to(TYPES[out]))
+    no_device_errors()
+
+
+def test_experts_slots_past_the_range_of_fp16():
+    """Slots beyond 65504, of both signs, whose weighted sums fit fp16."""
+    rng = np.random.default_rng(18)
+    E, H, I, k, N = 4, 200, 100, 2, 24
+    p, (gate, up, down) = layer(rng, E, H, I)
+    grow = 2.0 ** 22
+    p["down_q"] = (p["down_q"][0], p["down_q"][1] * grow)
+    down = [(q, s * np.float32(grow)) for q, s in down]
+    x = activations(rng, N, H, torch.bfloat16)
+    idx, w = gen.routing(rng, N, E, k)
+    one = np.ones((N, 1), np.float32)
+    slots = np.stack([fp8.experts(gate, up, down, f64(x), idx[:, j:j + 1], one, gen.LIMIT, 0.0)[0] for j in range(k)])
+    w = (w * np.float32(30000 / np.abs(slots).max())).astype(np.float32)
+    assert (slots.min(axis=0) < -65504).any() and (slots.max(axis=0) > 65504).any()
+    y = apply(p, x, idx, w, torch.float16)
+    want, bound = fp8.experts(gate, up, down, f64(x), idx, w.astype(np.float64), gen.LIMIT, half_eps(torch.float16))
+    # + half the least fp16 subnormal
+    assert torch.isfinite(y).all() and (np.abs(f64(y) - want) <= bound + 2.0 ** -25).all()
+    no_device_errors()
