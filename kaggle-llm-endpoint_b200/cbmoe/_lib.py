@@ -170,6 +170,12 @@ def require_cuda(*tensors):
     raise CbmoeError("cbmoe needs a CUDA device (no CPU fallback)")
 
 
+def no_gradient(name, *tensors):
+    """Refuses inputs that autograd follows: `name` has no backward pass, so their gradient would lack its part."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f"{name} has no gradient: detach its inputs or call it under torch.no_grad()")
+
+
 _same_device = contextlib.nullcontext()
 
 

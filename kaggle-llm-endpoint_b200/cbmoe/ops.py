@@ -7,7 +7,7 @@ import ctypes
 
 import torch
 
-from ._lib import E4M3, TYPES, check, lib, on_device, ptr, raw_stream, require_cuda, stream_handle
+from ._lib import E4M3, TYPES, check, lib, no_gradient, on_device, ptr, raw_stream, require_cuda, stream_handle
 
 PLAN_FIELDS = ("counts", "row_start", "act", "n_act", "n_blocks", "n_pass", "blk_expert", "tok_row", "w_row",
                "row_slot", "pass_expert", "pass_row0", "pass_cnt")
@@ -164,8 +164,10 @@ def _fp8_x(x):
 def fp8_quantize(x):
     """x [N, K] (bf16, fp16 or fp32) -> (q float8_e4m3fn [N, K], s fp32 [N, ceil(K / 128)]): per row and group of 128
     columns the scale is the least power of two s >= 2^-100 with max|x| <= 448 s, the codes e4m3(x / s). A group with
-    an infinity or a NaN has the scale NaN. q is a view of rows padded to 16 bytes, as fp8_linear takes it."""
+    an infinity or a NaN has the scale NaN. q is a view of rows padded to 16 bytes, as fp8_linear takes it. Has no
+    gradient: an x that requires one is refused."""
     require_cuda(x)
+    no_gradient("fp8_quantize", x)
     if x.dtype not in TYPES:
         raise ValueError(f"x is bf16, fp16 or fp32, got {x.dtype}")
     x, ldx = _fp8_x(x)
@@ -225,10 +227,11 @@ def fp8_linear(q, s, x, out_dtype=torch.float32):
     """x [N, K] @ W^T -> [N, rows] in out_dtype (fp32, bf16, fp16), W = e4m3 codes q [rows, K] (fp8_pad_rows) times fp32
     scales s [ceil(rows / 128), ceil(K / 128)] of 128 x 128 blocks. x: bf16, fp16 or fp32, quantised per row in groups of
     128 as fp8_quantize does, or the pair (codes, scales) that fp8_quantize returned (one quantisation for several
-    products). fp32 sums. Inference only: no gradient."""
+    products). fp32 sums. Inference only: inputs that require a gradient are refused."""
     ready = isinstance(x, (tuple, list))
     xv, xs = x if ready else (x, None)
     require_cuda(q, s, xv, xs)
+    no_gradient("fp8_linear", q, s, xv, xs)
     if q.dim() != 2 or xv.dim() != 2 or xv.shape[1] != q.shape[1] or q.shape[0] == 0 or q.shape[1] == 0:
         raise ValueError(f"q [rows, K] and x [N, K], got {tuple(q.shape)} and {tuple(xv.shape)}")
     if out_dtype not in TYPES:

@@ -430,3 +430,27 @@ def test_experts_slots_past_the_range_of_fp16():
     # + half the least fp16 subnormal
     assert torch.isfinite(y).all() and (np.abs(f64(y) - want) <= bound + 2.0 ** -25).all()
     no_device_errors()
+
+
+def test_inputs_that_require_a_gradient_are_refused():
+    """The products have no backward pass: under autograd they would drop their part of the gradient without a word."""
+    import cbmoe
+    rng = np.random.default_rng(20)
+    (q, s), _ = table(rng, 130, 256)
+    x = activations(rng, 4, 256, torch.float32).requires_grad_()
+    p, _ = layer(rng, 2, 256, 128)
+    idx, w = (torch.from_numpy(t).cuda() for t in gen.routing(rng, 4, 2, 2))
+    codes, scales = cbmoe.ops.fp8_quantize(x.detach())
+    fetch = cbmoe.ResidentFetch()
+    trained = w.clone().requires_grad_()
+    calls = (lambda: cbmoe.ops.fp8_linear(q, s, x), lambda: cbmoe.ops.fp8_quantize(x),
+             lambda: cbmoe.ops.fp8_linear(q, s.clone().requires_grad_(), x.detach()),
+             lambda: cbmoe.ops.fp8_linear(q, s, (codes, scales.clone().requires_grad_())),
+             lambda: fetch.apply(p, x, idx, w, 0, gen.LIMIT), lambda: fetch.apply(p, x.detach(), idx, trained, 0, gen.LIMIT))
+    for call in calls:
+        with pytest.raises(ValueError, match="no gradient"):
+            call()
+        with torch.no_grad():
+            call()
+    assert not fetch.apply(p, x.detach(), idx, w, 0, gen.LIMIT).requires_grad
+    no_device_errors()
