@@ -748,6 +748,7 @@ int launch_few(const Fp8Gemm& g, cudaStream_t s) {
 
 bool aligned(const void* p, int n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 bool type_ok(int t) { return t == CBMOE_BF16 || t == CBMOE_F16 || t == CBMOE_F32; }
+int elem_size(int t) { return t == CBMOE_F32 ? 4 : 2; }
 int blocks_of(int K) { return (K + kFp8Group - 1) / kFp8Group; }
 
 }  // namespace
@@ -780,7 +781,7 @@ int launch_fp8_quantize(const void* x, int type, int N, int K, long long ldx, ui
   const long long groups = (long long)N * blocks_of(K);
   long long blocks = (groups + 15) / 16, cap = (long long)num_sms() * 16;
   if (blocks > cap) blocks = cap;
-  const int size = type == CBMOE_F32 ? 4 : 2;
+  const int size = elem_size(type);
   const int vec = aligned(x, 16) && ldx * size % 16 == 0;
   prof_begin(kProfOther, stream);
   if (type == CBMOE_BF16)
@@ -868,7 +869,7 @@ extern "C" int cbmoe_fp8_quantize(const void* x, int type, int N, int K, long lo
                                   float* s, cudaStream_t stream) {
   if (!type_ok(type) || N < 0 || K <= 0 || ldx < K || ldq < K) return CBMOE_ERR_INVALID;
   if (N == 0) return CBMOE_OK;
-  if (!x || !q || !s) return CBMOE_ERR_INVALID;
+  if (!x || !q || !s || !aligned(x, elem_size(type)) || !aligned(s, 4)) return CBMOE_ERR_INVALID;
   return launch_fp8_quantize(x, type, N, K, ldx, q, ldq, s, blocks_of(K), nullptr, 1, N, 1, nullptr, 0, stream);
 }
 
@@ -885,7 +886,9 @@ extern "C" int cbmoe_fp8_linear(const void* q, long long ldq, const float* s, in
   if (!ready && !type_ok(x_type)) return CBMOE_ERR_INVALID;
   if (N == 0) return CBMOE_OK;
   if (N > (1 << 30) || K > (1 << 24)) return CBMOE_ERR_UNSUPPORTED;   // counts of tiles and blocks in 32 bits
-  if (!x || !y || ldx < K || (ready && (!xs || ldx % 16 || !aligned(x, 16)))) return CBMOE_ERR_INVALID;
+  if (!x || !y || ldx < K || !aligned(y, elem_size(y_type))) return CBMOE_ERR_INVALID;
+  if (ready ? !xs || ldx % 16 || !aligned(x, 16) || !aligned(xs, 4) : !aligned(x, elem_size(x_type)))
+    return CBMOE_ERR_INVALID;
   Fp8Gemm g{};
   g.rows = rows;
   g.K = K;
@@ -945,6 +948,7 @@ extern "C" int cbmoe_fp8_experts_apply(const cbmoe_fp8_experts* ex, const uint16
   if (!fp8_experts_ok(ex) || N < 0 || k <= 0 || k > 64 || !type_ok(y_type)) return CBMOE_ERR_INVALID;
   if (N == 0) return CBMOE_OK;
   if (!x || !idx || !w || !y) return CBMOE_ERR_INVALID;
+  if (!aligned(x, 2) || !aligned(idx, 4) || !aligned(w, 4) || !aligned(y, elem_size(y_type))) return CBMOE_ERR_INVALID;
   if ((long long)N * k > (1 << 30)) return CBMOE_ERR_UNSUPPORTED;
   const ExpertsWs W = experts_ws(ex->E, ex->H, ex->I, N, k);
   if (!workspace || workspace_bytes < W.total || !aligned(workspace, 256)) return CBMOE_ERR_WORKSPACE;

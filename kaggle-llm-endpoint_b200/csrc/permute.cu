@@ -312,6 +312,12 @@ int unpermute_backward_t(const void* dy, const void* ys, int R, int H, const int
 
 bool type_ok(int t) { return t == CBMOE_BF16 || t == CBMOE_F16 || t == CBMOE_F32; }
 
+// Elements of `size` bytes at each of the pointers.
+template <typename... P>
+bool aligned(size_t size, const P*... p) {
+  return ((reinterpret_cast<uintptr_t>(p) | ...) & (size - 1)) == 0;
+}
+
 }  // namespace
 
 // f<T, VB>(args...) for the type and the unit's bytes.
@@ -362,6 +368,7 @@ extern "C" int cbmoe_permute(const void* x, int type, int T, int H, const int32_
                              const int32_t* tok_row, int R, void* xs, cudaStream_t stream) {
   if (!type_ok(type) || T < 0 || H <= 0 || k <= 0 || R < 0) return CBMOE_ERR_INVALID;
   if ((T > 0 && (!x || !row_slot)) || (R > 0 && (!tok_row || !xs))) return CBMOE_ERR_INVALID;
+  if (!aligned(elem_size(type), x, xs) || !aligned(4, row_slot, tok_row)) return CBMOE_ERR_INVALID;
   if (R == 0) return CBMOE_OK;
   prof_begin(kProfOther, stream);
   const int rc = CBMOE_BY_TYPE(permute_t, type, unit_bytes(type, H, x, xs), x, T, H, row_slot, k, tok_row, R, xs, stream);
@@ -375,6 +382,7 @@ extern "C" int cbmoe_unpermute(const void* ys, int type, int R, int H, const int
                                int k, void* y, cudaStream_t stream) {
   if (!type_ok(type) || T < 0 || H <= 0 || k <= 0 || R < 0) return CBMOE_ERR_INVALID;
   if (T > 0 && (!row_slot || !y || (R > 0 && !ys))) return CBMOE_ERR_INVALID;
+  if (!aligned(elem_size(type), ys, y) || !aligned(4, row_slot, w)) return CBMOE_ERR_INVALID;
   if (T == 0) return CBMOE_OK;
   prof_begin(kProfCombine, stream);
   const int rc = CBMOE_BY_TYPE(unpermute_t, type, unit_bytes(type, H, ys, y), ys, R, H, row_slot, w, T, k, y, stream);
@@ -389,6 +397,7 @@ extern "C" int cbmoe_unpermute_backward(const void* dy, const void* ys, int type
                                         void* dys, float* dw, cudaStream_t stream) {
   if (!type_ok(type) || T < 0 || H <= 0 || k <= 0 || R < 0) return CBMOE_ERR_INVALID;
   if ((T > 0 && (!dy || !row_slot)) || (dw && R > 0 && !ys) || (dys && R > 0 && !tok_row)) return CBMOE_ERR_INVALID;
+  if (!aligned(elem_size(type), dy, ys, dys) || !aligned(4, row_slot, tok_row, w, dw)) return CBMOE_ERR_INVALID;
   if (!dys && !dw) return CBMOE_OK;
   if (T == 0 && (!dys || R == 0)) return CBMOE_OK;
   prof_begin(kProfCombine, stream);

@@ -121,3 +121,41 @@ def test_row_padding_of_codes():
     assert ops.fp8_row_stride(whole[:, :, 16:]) == 32 and ops.fp8_row_stride(whole[:, :, 8:]) is None
     with pytest.raises(ValueError):
         ops.fp8_pad_rows(raw.view(3, 20))
+
+
+def token_order(L, t):
+    """The three entry points for elements of type t, with defaults that they take up to the launch."""
+    def permute(x=16, T=2, H=8, slot=16, k=2, tok=16, R=4, xs=16):
+        return L.cbmoe_permute(x, t, T, H, slot, k, tok, R, xs, None)
+
+    def unpermute(ys=16, R=4, H=8, slot=16, w=16, T=2, k=2, y=16):
+        return L.cbmoe_unpermute(ys, t, R, H, slot, w, T, k, y, None)
+
+    def backward(dy=16, ys=16, R=4, H=8, slot=16, tok=16, w=16, T=2, k=2, dys=16, dw=16):
+        return L.cbmoe_unpermute_backward(dy, ys, t, R, H, slot, tok, w, T, k, dys, dw, None)
+
+    return permute, unpermute, backward
+
+
+def test_misaligned_elements_are_refused(L):
+    """A pointer off its element's alignment would be a misaligned address in the kernel."""
+    from cbmoe._lib import Fp8Experts
+    for t, size in ((BF16, 2), (F16, 2), (F32, 4)):
+        permute, unpermute, backward = token_order(L, t)
+        for f, typed, words in ((permute, ("x", "xs"), ("slot", "tok")), (unpermute, ("ys", "y"), ("slot", "w")),
+                                (backward, ("dy", "ys", "dys"), ("slot", "tok", "w", "dw"))):
+            for name in typed:
+                assert f(**{name: 16 + size // 2}) == INVALID, (f, name)
+            for name in words:
+                assert f(**{name: 18}) == INVALID, (f, name)
+        assert L.cbmoe_fp8_quantize(16 + size // 2, t, 1, 128, 128, 16, 128, 16, None) == INVALID
+        assert linear(L, x=16 + size // 2, x_type=t) == INVALID
+        assert linear(L, y=16 + size // 2, y_type=t) == INVALID
+    assert L.cbmoe_fp8_quantize(16, BF16, 1, 128, 128, 17, 128, 18, None) == INVALID              # s
+    assert linear(L, x_type=E4M3, xs=18) == INVALID
+    ex = Fp8Experts(E=4, H=256, I=128, gate=16, up=16, down=16, gate_s=16, up_s=16, down_s=16, ld_in=256, ld_down=128)
+    good = dict(x=16, idx=16, w=16, y=16, y_type=F32)
+    for bad in (dict(x=17), dict(idx=18), dict(w=18), dict(y=18), dict(y=17, y_type=BF16)):
+        a = {**good, **bad}
+        assert L.cbmoe_fp8_experts_apply(ctypes.byref(ex), a["x"], 1, a["idx"], a["w"], 2, 10.0, a["y"], a["y_type"], 256,
+                                         1 << 30, None) == INVALID, bad
