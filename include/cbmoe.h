@@ -236,8 +236,8 @@ int cbmoe_route(const uint16_t* x, int N, int D, const uint16_t* router_w, const
  * multiple of 16, >= K) is an argument, the first row 16-byte aligned, the scales dense. Activations are quantised per
  * row in groups of 128 columns: scale = the least power of two s >= 2^-100 with max|x| <= 448 s, codes = e4m3(x / s)
  * (an exact division; round to nearest even); a group that holds an infinity or a NaN has the scale NaN and stands for
- * NaN, so the row's products are NaN. Any rows >= 1 and K >= 1 (products: K <= 2^24, N <= 2^30): sizes need not be multiples of
- * anything.
+ * NaN, so the row's products are NaN. Any rows >= 1 and K >= 1 (quantiser: K <= 2^30; products: K <= 2^24, N <= 2^30):
+ * sizes need not be multiples of anything.
  * No counterpart in the reference, which converts such weights to other formats at load time. */
 /* x [N][K] of `type` (CBMOE_BF16 / F16 / F32; row stride ldx elements) -> q [N][K] e4m3 (row stride ldq bytes; bytes
  * between K and ldq may be written with zeros) and s fp32 [N][ceil(K/128)]. */
@@ -275,7 +275,7 @@ int cbmoe_fp8_experts_apply(const cbmoe_fp8_experts* ex, const uint16_t* x, int 
 /* ------------------------------------------------------------------- tokens into expert order and back
  * Over a routing plan's row_slot [T][k] (a slot's sorted row; outside [0, R): empty) and tok_row [R] (a sorted row's
  * token; < 0: padding). Element type CBMOE_BF16 / F16 / F32, rows dense [.][H], any H; sums in fp32 over j in order,
- * rounded once, no atomics. Pointers are aligned to their elements. The row gather and the combine of
+ * rounded once, no atomics. Pointers are aligned to their elements; T, R, H, k <= 2^31 - 2^16. The row gather and the combine of
  * resident.py:144-165 as operators, with gradients. */
 /* xs[row_slot[t][j]] = x[t]; rows with tok_row < 0 are zero. Its gradient is cbmoe_unpermute with w NULL. */
 int cbmoe_permute(const void* x, int type, int T, int H, const int32_t* row_slot, int k, const int32_t* tok_row, int R,

@@ -176,6 +176,13 @@ def no_gradient(name, *tensors):
         raise ValueError(f"{name} has no gradient: detach its inputs or call it under torch.no_grad()")
 
 
+def int_sizes(*tensors):
+    """Refuses shapes whose sizes do not fit the library's 32-bit counts (a C int would silently take other ones)."""
+    for t in tensors:
+        if t is not None and max(t.shape, default=0) > 0x7fffffff:
+            raise ValueError(f"sizes up to 2^31 - 1 are supported, got {tuple(t.shape)}")
+
+
 _same_device = contextlib.nullcontext()
 
 

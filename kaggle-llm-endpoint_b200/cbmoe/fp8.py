@@ -10,7 +10,7 @@ Activations are quantised per row in groups of 128 (ops.fp8_quantize); so is the
 import torch
 
 from . import ops
-from ._lib import TYPES, Fp8Experts, check, lib, no_gradient, on_device, raw_stream, require_cuda
+from ._lib import TYPES, Fp8Experts, check, int_sizes, lib, no_gradient, on_device, raw_stream, require_cuda
 
 FP8 = "FP8"
 
@@ -21,6 +21,7 @@ def pack_layer(gate, up, down):
     ResidentFetch.apply takes. Codes whose rows are 16-byte aligned are kept as they are, others get a padded copy."""
     (gq, gs), (uq, us), (dq, ds) = gate, up, down
     require_cuda(gq, gs, uq, us, dq, ds)
+    int_sizes(gq, uq, dq)
     if gq.dim() != 3 or 0 in gq.shape:
         raise ValueError(f"gate codes are [E, I, H], got {tuple(gq.shape)}")
     E, I, H = gq.shape
@@ -44,6 +45,7 @@ def apply(p, x, idx, w, limit, out_dtype=torch.float32):
     """x bf16 [N, H]; idx int32 [N, k]; w fp32 [N, k] -> the routed partial [N, H] in out_dtype (fp32, bf16, fp16).
     Inference only: inputs that require a gradient are refused."""
     no_gradient("the expert layer on FP8 tables", x, w, *(t for n in ("gate_q", "up_q", "down_q") for t in p[n]))
+    int_sizes(idx)
     N, k = idx.shape
     if out_dtype not in TYPES:
         raise ValueError(f"out_dtype is fp32, bf16 or fp16, got {out_dtype}")

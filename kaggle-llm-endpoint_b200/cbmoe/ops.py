@@ -7,7 +7,8 @@ import ctypes
 
 import torch
 
-from ._lib import E4M3, TYPES, check, lib, no_gradient, on_device, ptr, raw_stream, require_cuda, stream_handle
+from ._lib import (E4M3, TYPES, check, int_sizes, lib, no_gradient, on_device, ptr, raw_stream, require_cuda,
+                   stream_handle)
 
 PLAN_FIELDS = ("counts", "row_start", "act", "n_act", "n_blocks", "n_pass", "blk_expert", "tok_row", "w_row",
                "row_slot", "pass_expert", "pass_row0", "pass_cnt")
@@ -168,6 +169,7 @@ def fp8_quantize(x):
     gradient: an x that requires one is refused."""
     require_cuda(x)
     no_gradient("fp8_quantize", x)
+    int_sizes(x)
     if x.dtype not in TYPES:
         raise ValueError(f"x is bf16, fp16 or fp32, got {x.dtype}")
     x, ldx = _fp8_x(x)
@@ -232,6 +234,7 @@ def fp8_linear(q, s, x, out_dtype=torch.float32):
     xv, xs = x if ready else (x, None)
     require_cuda(q, s, xv, xs)
     no_gradient("fp8_linear", q, s, xv, xs)
+    int_sizes(q, xv)
     if q.dim() != 2 or xv.dim() != 2 or xv.shape[1] != q.shape[1] or q.shape[0] == 0 or q.shape[1] == 0:
         raise ValueError(f"q [rows, K] and x [N, K], got {tuple(q.shape)} and {tuple(xv.shape)}")
     if out_dtype not in TYPES:

@@ -11,7 +11,7 @@ backward give the same bits on every call.
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._lib import TYPES, check, lib, on_device, raw_stream, require_cuda
+from ._lib import TYPES, check, int_sizes, lib, on_device, raw_stream, require_cuda
 
 
 def _ptr(t):
@@ -25,6 +25,7 @@ def _plan_rows(plan, device):
         if t.dtype is not torch.int32 or t.dim() != dim or not t.is_contiguous() or t.device != device:
             raise ValueError(f"plan[{name!r}] is contiguous int32 of {dim} dimension(s) on {device}, got {t.dtype} "
                              f"{tuple(t.shape)} on {t.device}")
+    int_sizes(tok_row, row_slot)
     if row_slot.shape[1] == 0:
         raise ValueError("the plan has no slots per token")
     blocks = plan.get("blk_expert")
@@ -35,6 +36,7 @@ def _plan_rows(plan, device):
 
 def _rows(name, t):
     require_cuda(t)
+    int_sizes(t)
     if t.dim() != 2 or t.shape[1] == 0:
         raise ValueError(f"{name} is [rows, H], got {tuple(t.shape)}")
     if t.dtype not in TYPES:

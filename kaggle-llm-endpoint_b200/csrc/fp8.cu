@@ -870,6 +870,7 @@ extern "C" int cbmoe_fp8_quantize(const void* x, int type, int N, int K, long lo
   if (!type_ok(type) || N < 0 || K <= 0 || ldx < K || ldq < K) return CBMOE_ERR_INVALID;
   if (N == 0) return CBMOE_OK;
   if (!x || !q || !s || !aligned(x, elem_size(type)) || !aligned(s, 4)) return CBMOE_ERR_INVALID;
+  if (K > (1 << 30)) return CBMOE_ERR_UNSUPPORTED;                    // columns in 32 bits
   return launch_fp8_quantize(x, type, N, K, ldx, q, ldq, s, blocks_of(K), nullptr, 1, N, 1, nullptr, 0, stream);
 }
 

@@ -318,6 +318,13 @@ bool aligned(size_t size, const P*... p) {
   return ((reinterpret_cast<uintptr_t>(p) | ...) & (size - 1)) == 0;
 }
 
+// The kernels' strided loops count in 32 bits: a count and the largest step (a row's columns over 2 * 148 blocks of 128
+// threads) stay below 2^31.
+bool counts_ok(int T, int R, int H, int k) {
+  constexpr int kMost = 0x7fff0000;
+  return T <= kMost && R <= kMost && H <= kMost && k <= kMost;
+}
+
 }  // namespace
 
 // f<T, VB>(args...) for the type and the unit's bytes.
@@ -369,6 +376,7 @@ extern "C" int cbmoe_permute(const void* x, int type, int T, int H, const int32_
   if (!type_ok(type) || T < 0 || H <= 0 || k <= 0 || R < 0) return CBMOE_ERR_INVALID;
   if ((T > 0 && (!x || !row_slot)) || (R > 0 && (!tok_row || !xs))) return CBMOE_ERR_INVALID;
   if (!aligned(elem_size(type), x, xs) || !aligned(4, row_slot, tok_row)) return CBMOE_ERR_INVALID;
+  if (!counts_ok(T, R, H, k)) return CBMOE_ERR_UNSUPPORTED;
   if (R == 0) return CBMOE_OK;
   prof_begin(kProfOther, stream);
   const int rc = CBMOE_BY_TYPE(permute_t, type, unit_bytes(type, H, x, xs), x, T, H, row_slot, k, tok_row, R, xs, stream);
@@ -383,6 +391,7 @@ extern "C" int cbmoe_unpermute(const void* ys, int type, int R, int H, const int
   if (!type_ok(type) || T < 0 || H <= 0 || k <= 0 || R < 0) return CBMOE_ERR_INVALID;
   if (T > 0 && (!row_slot || !y || (R > 0 && !ys))) return CBMOE_ERR_INVALID;
   if (!aligned(elem_size(type), ys, y) || !aligned(4, row_slot, w)) return CBMOE_ERR_INVALID;
+  if (!counts_ok(T, R, H, k)) return CBMOE_ERR_UNSUPPORTED;
   if (T == 0) return CBMOE_OK;
   prof_begin(kProfCombine, stream);
   const int rc = CBMOE_BY_TYPE(unpermute_t, type, unit_bytes(type, H, ys, y), ys, R, H, row_slot, w, T, k, y, stream);
@@ -398,6 +407,7 @@ extern "C" int cbmoe_unpermute_backward(const void* dy, const void* ys, int type
   if (!type_ok(type) || T < 0 || H <= 0 || k <= 0 || R < 0) return CBMOE_ERR_INVALID;
   if ((T > 0 && (!dy || !row_slot)) || (dw && R > 0 && !ys) || (dys && R > 0 && !tok_row)) return CBMOE_ERR_INVALID;
   if (!aligned(elem_size(type), dy, ys, dys) || !aligned(4, row_slot, tok_row, w, dw)) return CBMOE_ERR_INVALID;
+  if (!counts_ok(T, R, H, k)) return CBMOE_ERR_UNSUPPORTED;
   if (!dys && !dw) return CBMOE_OK;
   if (T == 0 && (!dys || R == 0)) return CBMOE_OK;
   prof_begin(kProfCombine, stream);

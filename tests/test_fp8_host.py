@@ -159,3 +159,24 @@ def test_misaligned_elements_are_refused(L):
         a = {**good, **bad}
         assert L.cbmoe_fp8_experts_apply(ctypes.byref(ex), a["x"], 1, a["idx"], a["w"], 2, 10.0, a["y"], a["y_type"], 256,
                                          1 << 30, None) == INVALID, bad
+
+
+def test_counts_past_32_bit_loops_are_refused(L):
+    """The kernels' strided loops count in 32 bits: tokens, rows, widths and slots a token up to 2^31 - 2^16 stay in range."""
+    most, past = 0x7fff0000, 0x7fff0001
+    for t in (BF16, F16, F32):
+        permute, unpermute, backward = token_order(L, t)
+        for f in (permute, unpermute, backward):
+            for name in ("T", "R", "H", "k"):
+                assert f(**{name: past}) == UNSUPPORTED, (f, name)
+        assert permute(T=most, R=0) == 0 and unpermute(T=0, R=most) == 0 and backward(T=most, dys=None, dw=None) == 0
+        assert L.cbmoe_fp8_quantize(16, t, 1, (1 << 30) + 1, 1 << 31, 16, 1 << 31, 16, None) == UNSUPPORTED
+
+
+def test_shapes_past_32_bits_are_refused():
+    """Sizes that a C int would cut to other ones raise; meta tensors stand for tensors that need no memory."""
+    from cbmoe import _lib
+    for shape in ((1, (1 << 32) + 8), ((1 << 31), 1), (0, 1 << 31)):
+        with pytest.raises(ValueError):
+            _lib.int_sizes(torch.empty(shape, device="meta", dtype=torch.bfloat16))
+    _lib.int_sizes(torch.empty(3, (1 << 31) - 1, device="meta"), None)
