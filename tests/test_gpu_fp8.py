@@ -454,3 +454,56 @@ def test_inputs_that_require_a_gradient_are_refused():
             call()
     assert not fetch.apply(p, x.detach(), idx, w, 0, gen.LIMIT).requires_grad
     no_device_errors()
+
+
+@pytest.fixture(scope="module")
+def wide_layer():
+    """40 experts of 4 gate/up tiles (10 column blocks each): more tiles than SMs whatever the rows of a pass."""
+    rng = np.random.default_rng(19)
+    return layer(rng, 40, 1280, 512)
+
+
+@pytest.mark.parametrize("N,skew,width", [(60, False, 32), (400, False, 64), (900, False, 128), (1500, False, 256),
+                                          (60, True, 32), (1604, True, 256)])
+def test_experts_with_more_tiles_than_sms(wide_layer, N, skew, width):
+    """Passes of 32, 64, 128 and 256 rows, where a CTA (at 256 rows: a pair) takes several tiles one after another; pairs
+    cut the gate/up tiles left over along K. Skewed: one expert has a slot of every token, a few rows past whole passes."""
+    p, (gate, up, down) = wide_layer
+    E, H, I, k = 40, 1280, 512, 4
+    rng = np.random.default_rng(N + skew)
+    x = activations(rng, N, H, torch.bfloat16)
+    idx, w = gen.routing(rng, N, E, k)
+    if skew:
+        idx[idx == 7] = 8
+        idx[:, 0] = 7
+    slots = N * k / E
+    assert width == (32 if slots <= 32 else 64 if slots <= 64 else 128 if slots <= 128 else 256)
+    counts = np.bincount(idx.ravel(), minlength=E)
+    tiles = int((-(-counts // width)).sum()) * (I // 128)
+    workers = torch.cuda.get_device_properties(0).multi_processor_count // (2 if width == 256 else 1)
+    assert tiles > workers and (width < 256 or tiles % workers)
+    want, bound = fp8.experts(gate, up, down, f64(x), idx, w.astype(np.float64), gen.LIMIT, half_eps(torch.float32))
+    y = apply(p, x, idx, w, torch.float32)
+    assert (np.abs(f64(y) - want) <= bound).all()
+    assert np.linalg.norm(f64(y) - want) <= 2.0 ** -5.5 * np.linalg.norm(want)     # as in test_experts_match_oracle
+    assert torch.equal(apply(p, x, idx, w, torch.float32), y)
+    no_device_errors()
+
+
+@pytest.mark.parametrize("N,K,rows", [(3, 8192, 262400), (262400, 8192, 130), (70000, 130, 32768)])
+def test_linear_past_32_bit_offsets(N, K, rows):
+    """Weights, activations and outputs of more than 2^31 elements: the last rows are found where they lie."""
+    import cbmoe
+    g = torch.Generator(device="cuda").manual_seed(N)
+    ld = -(-K // 16) * 16
+    q = torch.randint(0, 0x7F, (rows, ld), dtype=torch.uint8, device="cuda", generator=g).view(torch.float8_e4m3fn)[:, :K]
+    s = torch.rand(-(-rows // 128), -(-K // 128), device="cuda", generator=g) * 2.0 ** -10
+    x = torch.randn(N, K, device="cuda", generator=g, dtype=torch.bfloat16)
+    y = cbmoe.ops.fp8_linear(q, s, x, out_dtype=torch.bfloat16)
+    n = torch.tensor(sorted({0, N // 2, N - 2, N - 1}), device="cuda")
+    b = sorted({0, rows // 128 // 2, -(-rows // 128) - 1})                       # 128-row blocks
+    for i in b:
+        r = slice(128 * i, min(128 * i + 128, rows))
+        want, bound = fp8.linear(f64(q[r].float()), f64(s[i:i + 1]), f64(x[n]), half_eps(torch.bfloat16))
+        assert (np.abs(f64(y[n, r]) - want) <= bound).all()
+    no_device_errors()

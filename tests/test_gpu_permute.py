@@ -240,3 +240,28 @@ def test_refusals():
                  lambda: p(x, {**plan, "row_slot": plan["row_slot"].t()})):
         with pytest.raises(ValueError):
             call()
+
+
+def test_rows_past_32_bit_offsets():
+    """More than 2^31 elements of sorted rows: permute, its gradient and unpermute find the last rows where they lie."""
+    import cbmoe
+    T, H, E, k = 33000, 32776, 4, 2
+    g = torch.Generator(device="cuda").manual_seed(3)
+    idx = torch.randint(0, E, (T, k), device="cuda", generator=g, dtype=torch.int32)
+    w = torch.ones(T, k, device="cuda")
+    plan = cbmoe.ops.route_plan(idx, w, E, 1)
+    x = torch.randint(-3, 4, (T, H), device="cuda", generator=g).to(torch.bfloat16)
+    slot = plan["row_slot"].long()
+    xs = cbmoe.moe_permute(x, plan)
+    assert xs.shape == (T * k, H) and xs.numel() > 1 << 31
+    for rows in torch.arange(T, device="cuda").split(4000):
+        assert torch.equal(xs[slot[rows, 0]], x[rows]) and torch.equal(xs[slot[rows, 1]], x[rows])
+    y = cbmoe.moe_unpermute(xs, w, plan)                      # whole numbers: x + x without rounding
+    assert torch.equal(y, x + x)
+    del y
+    ys = xs.requires_grad_()
+    wl = w.clone().requires_grad_()
+    dys, dw = torch.autograd.grad(cbmoe.moe_unpermute(ys, wl, plan), (ys, wl), x)
+    assert torch.equal(dys, xs.detach())
+    want = torch.cat([x[r].float().square().sum(1) for r in torch.arange(T, device="cuda").split(4000)])
+    assert torch.equal(dw, want[:, None].expand(T, k))        # sums of whole numbers below 2^24: exact
