@@ -172,15 +172,16 @@ def require_cuda(*tensors):
 
 def no_gradient(name, *tensors):
     """Refuses inputs that autograd follows: `name` has no backward pass, so their gradient would lack its part."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{name} has no gradient: detach its inputs or call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{name} has no gradient: detach its inputs or call it under torch.no_grad()")
 
 
-def int_sizes(*tensors):
-    """Refuses shapes whose sizes do not fit the library's 32-bit counts (a C int would silently take other ones)."""
-    for t in tensors:
-        if t is not None and max(t.shape, default=0) > 0x7fffffff:
-            raise ValueError(f"sizes up to 2^31 - 1 are supported, got {tuple(t.shape)}")
+def int_sizes(*sizes):
+    """Refuses sizes that do not fit the library's 32-bit counts (a C int would silently take other ones)."""
+    if max(sizes) > 0x7fffffff:
+        raise ValueError(f"sizes up to 2^31 - 1 are supported, got {max(sizes)}")
 
 
 _same_device = contextlib.nullcontext()

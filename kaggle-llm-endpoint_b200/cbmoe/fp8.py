@@ -21,10 +21,10 @@ def pack_layer(gate, up, down):
     ResidentFetch.apply takes. Codes whose rows are 16-byte aligned are kept as they are, others get a padded copy."""
     (gq, gs), (uq, us), (dq, ds) = gate, up, down
     require_cuda(gq, gs, uq, us, dq, ds)
-    int_sizes(gq, uq, dq)
     if gq.dim() != 3 or 0 in gq.shape:
         raise ValueError(f"gate codes are [E, I, H], got {tuple(gq.shape)}")
     E, I, H = gq.shape
+    int_sizes(E, I, H)
     gq, uq, dq = (ops.fp8_pad_rows(t) for t in (gq, uq, dq))
     gs, us, ds = (t.contiguous() for t in (gs, us, ds))
     ld = [ops.fp8_table_stride(n, q, s, (E,), r, c, gq.device)
@@ -45,8 +45,8 @@ def apply(p, x, idx, w, limit, out_dtype=torch.float32):
     """x bf16 [N, H]; idx int32 [N, k]; w fp32 [N, k] -> the routed partial [N, H] in out_dtype (fp32, bf16, fp16).
     Inference only: inputs that require a gradient are refused."""
     no_gradient("the expert layer on FP8 tables", x, w, *(t for n in ("gate_q", "up_q", "down_q") for t in p[n]))
-    int_sizes(idx)
     N, k = idx.shape
+    int_sizes(N, k)
     if out_dtype not in TYPES:
         raise ValueError(f"out_dtype is fp32, bf16 or fp16, got {out_dtype}")
     if not p["gate_q"][0].device == x.device == idx.device == w.device:

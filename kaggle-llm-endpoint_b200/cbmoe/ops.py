@@ -169,11 +169,11 @@ def fp8_quantize(x):
     gradient: an x that requires one is refused."""
     require_cuda(x)
     no_gradient("fp8_quantize", x)
-    int_sizes(x)
     if x.dtype not in TYPES:
         raise ValueError(f"x is bf16, fp16 or fp32, got {x.dtype}")
     x, ldx = _fp8_x(x)
     N, K = x.shape
+    int_sizes(N, K)
     if K == 0:
         raise ValueError("x has no columns")
     ld = -(-K // 16) * 16
@@ -234,12 +234,12 @@ def fp8_linear(q, s, x, out_dtype=torch.float32):
     xv, xs = x if ready else (x, None)
     require_cuda(q, s, xv, xs)
     no_gradient("fp8_linear", q, s, xv, xs)
-    int_sizes(q, xv)
     if q.dim() != 2 or xv.dim() != 2 or xv.shape[1] != q.shape[1] or q.shape[0] == 0 or q.shape[1] == 0:
         raise ValueError(f"q [rows, K] and x [N, K], got {tuple(q.shape)} and {tuple(xv.shape)}")
     if out_dtype not in TYPES:
         raise ValueError(f"out_dtype is fp32, bf16 or fp16, got {out_dtype}")
     (rows, K), N = q.shape, xv.shape[0]
+    int_sizes(rows, K, N)
     ldq = fp8_table_stride("weights", q, s, (), rows, K, xv.device)
     if ready:
         if xv.dtype != torch.float8_e4m3fn:

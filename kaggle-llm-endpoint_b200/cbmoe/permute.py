@@ -25,7 +25,7 @@ def _plan_rows(plan, device):
         if t.dtype is not torch.int32 or t.dim() != dim or not t.is_contiguous() or t.device != device:
             raise ValueError(f"plan[{name!r}] is contiguous int32 of {dim} dimension(s) on {device}, got {t.dtype} "
                              f"{tuple(t.shape)} on {t.device}")
-    int_sizes(tok_row, row_slot)
+    int_sizes(*tok_row.shape, *row_slot.shape)
     if row_slot.shape[1] == 0:
         raise ValueError("the plan has no slots per token")
     blocks = plan.get("blk_expert")
@@ -36,9 +36,9 @@ def _plan_rows(plan, device):
 
 def _rows(name, t):
     require_cuda(t)
-    int_sizes(t)
     if t.dim() != 2 or t.shape[1] == 0:
         raise ValueError(f"{name} is [rows, H], got {tuple(t.shape)}")
+    int_sizes(*t.shape)
     if t.dtype not in TYPES:
         raise ValueError(f"{name} is bf16, fp16 or fp32, got {t.dtype}")
 
