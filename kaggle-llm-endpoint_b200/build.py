@@ -3,8 +3,9 @@
     python kaggle-llm-endpoint_b200/build.py          # -> kaggle-llm-endpoint_b200/cbmoe/libcbmoe.so
 
 Every .cu under csrc/ is compiled with relocatable device code (one device symbol, the error word, is shared
-across files; OWN_UNIT below names the exceptions) and linked into one shared library with the CUDA runtime linked statically. Objects go to
-_build/ next to this file; a file is recompiled when it or any header under csrc/ or include/ is newer.
+across files; OWN_UNIT below names the exceptions) and linked into one shared library with the CUDA runtime linked
+statically. Objects go to _build/ next to this file; a file is recompiled when it or any header under csrc/ or include/ is
+newer.
 """
 import glob
 import os

@@ -154,9 +154,15 @@ def stream_handle(device=None):
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+# torch's own lookup of a device's current stream as a plain handle, without the Stream object that the public call makes.
+# Not part of torch's public interface, so the public call stands in where a torch has none.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def raw_stream(t):
     """The current stream of t's device as a plain handle."""
-    return torch._C._cuda_getCurrentRawStream(t.device.index)
+    return _raw_stream(t.device.index)
 
 
 def require_cuda(*tensors):

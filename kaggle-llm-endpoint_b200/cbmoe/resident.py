@@ -60,9 +60,11 @@ class ResidentFetch:
     """Stored on the engine; `apply(p, x, idx, w, layer, limit)` as in resident.py:100-108.
 
     Constructor knobs keep the reference's names: `qtypes` {layer: {"gate_q", "up_q", "down_q"} -> format}
-    ("CB3" only here; the GGUF formats of cbmoe.iq and "FP8" of cbmoe.fp8 by their tables), `D`, `ml` (this GPU's intermediate size), `out_dtype` of the returned partial,
-    `gather_max_rows` (slots N*k at or below which the decode kernels run; above it the grouped path), and
-    `path` to force "decode" or "grouped"."""
+    ("CB3" only here; the GGUF formats of cbmoe.iq and "FP8" of cbmoe.fp8 by their tables), `D`, `ml` (this GPU's
+    intermediate size), `out_dtype` of the returned partial, `gather_max_rows` (slots N*k at or below which the decode
+    kernels run; above it the grouped path), and `path` to force "decode" or "grouped". These two choose between the CB3
+    kernels; the GGUF and FP8 formats have one path for every size and take no notice of them. `layer` and `moe_dense`
+    take CB3 tables with a shared expert only."""
 
     def __init__(self, qtypes=None, D=None, ml=None, out_dtype=torch.float32, gather_max_rows=1024, path="auto"):
         self.qtypes = qtypes or {}
