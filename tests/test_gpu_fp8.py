@@ -507,3 +507,16 @@ def test_linear_past_32_bit_offsets(N, K, rows):
         want, bound = fp8.linear(f64(q[r].float()), f64(s[i:i + 1]), f64(x[n]), half_eps(torch.bfloat16))
         assert (np.abs(f64(y[n, r]) - want) <= bound).all()
     no_device_errors()
+
+
+def test_weights_of_empty_slots_are_not_read():
+    rng = np.random.default_rng(21)
+    p, _ = layer(rng, 5, 200, 130)
+    x = activations(rng, 40, 200, torch.bfloat16)
+    idx, w = gen.routing(rng, 40, 5, 3)
+    idx[rng.random(idx.shape) < 0.4] = -1
+    want = apply(p, x, idx, w, torch.bfloat16)
+    w[idx < 0] = np.nan
+    y = apply(p, x, idx, w, torch.bfloat16)
+    assert torch.isfinite(y).all() and torch.equal(y, want)
+    no_device_errors()

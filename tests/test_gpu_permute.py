@@ -265,3 +265,24 @@ def test_rows_past_32_bit_offsets():
     assert torch.equal(dys, xs.detach())
     want = torch.cat([x[r].float().square().sum(1) for r in torch.arange(T, device="cuda").split(4000)])
     assert torch.equal(dw, want[:, None].expand(T, k))        # sums of whole numbers below 2^24: exact
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_infinities_and_nans_in_masked_places(dtype):
+    """Padding rows of ys and of permute's incoming gradient, and the weights of empty slots, are never read."""
+    import cbmoe
+    T, E, k, H, tm = 29, 5, 4, 70, 8
+    plan, idx, w, new = case(T, E, k, H, tm, dtype, True)
+    pad, empty = plan["tok_row"] < 0, plan["row_slot"] < 0
+    x, ys, dy, g = new(T, H).requires_grad_(), new(pad.numel(), H), new(T, H), new(pad.numel(), H)
+    bad_ys, bad_g, bad_w = ys.clone(), g.clone(), w.clone()
+    bad_ys[pad], bad_g[pad] = float("nan"), float("-inf")
+    bad_w[empty] = float("nan")
+    ys[pad], w[empty] = 0, 0
+    got = []
+    for a, b, wl in ((ys, g, w), (bad_ys, bad_g, bad_w)):
+        a, wl = a.clone().requires_grad_(), wl.clone().requires_grad_()
+        y = cbmoe.moe_unpermute(a, wl, plan)
+        got.append([y, *torch.autograd.grad(y, (a, wl), dy),
+                    *torch.autograd.grad(cbmoe.moe_permute(x, plan), x, b)])
+    assert all(torch.isfinite(t).all() and torch.equal(s, t) for s, t in zip(*got))
