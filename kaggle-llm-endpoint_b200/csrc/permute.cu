@@ -9,7 +9,7 @@
 // sorted rows are written (or read) once, and no row is touched twice. A sorted row belongs to one slot, so nothing is
 // added by atomics: sums run over j in order, in fp32, rounded once. Rows outside [0, R) in row_slot are empty slots.
 // Measured on one B200, 4096 tokens x 8 slots, rows of 5120 bf16 (about 375 MB a direction, 57 us at the copy rate):
-// permute 67 us, unpermute 70 us; backward of the weighted form 150 us for 108 us of bytes (it reads ys and writes dys).
+// permute 67 us, unpermute 68 us; backward of the weighted form 150 us for 108 us of bytes (it reads ys and writes dys).
 // Looking a slot's row up once per token and not once per unit took the plan, permute and its gradient from 198 to 184 us.
 #include <cuda_fp16.h>
 
@@ -351,6 +351,7 @@ int unpermute_to_f16(const void* ys, int R, int H, const int32_t* row_slot, cons
 
 }  // namespace
 
+// The expert layer's combine: fp32 slots, y in any type. 4096 x 8 rows of 5120 into fp32: 130 us, 115 at the copy rate.
 int launch_unpermute_f32(const float* ys, int R, int H, const int32_t* row_slot, const float* w, int T, int k, void* y,
                          int y_type, cudaStream_t stream) {
   // 16-bit rows of y are half as wide as those of ys: a unit of y is aligned where twice its address is
