@@ -275,8 +275,8 @@ int cbmoe_fp8_experts_apply(const cbmoe_fp8_experts* ex, const uint16_t* x, int 
 /* ------------------------------------------------------------------- tokens into expert order and back
  * Over a routing plan's row_slot [T][k] (a slot's sorted row; outside [0, R): empty) and tok_row [R] (a sorted row's
  * token; < 0: padding). Element type CBMOE_BF16 / F16 / F32, rows dense [.][H], any H; sums in fp32 over j in order,
- * rounded once, no atomics. Pointers are aligned to their elements; T, R, H, k <= 2^31 - 2^16. The row gather and the combine of
- * resident.py:144-165 as operators, with gradients. */
+ * rounded once, no atomics. Pointers are aligned to their elements; T, R, H, k <= 2^31 - 2^16. The row gather and the
+ * combine of resident.py:144-165 as operators, with gradients. */
 /* xs[row_slot[t][j]] = x[t]; rows with tok_row < 0 are zero. Its gradient is cbmoe_unpermute with w NULL. */
 int cbmoe_permute(const void* x, int type, int T, int H, const int32_t* row_slot, int k, const int32_t* tok_row, int R,
                   void* xs, cudaStream_t stream);
